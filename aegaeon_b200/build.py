@@ -21,11 +21,14 @@ SOURCES = [
     os.path.join(HERE, "csrc", "kvx_noalloc.cu"),
     os.path.join(HERE, "csrc", "kvx_safetensors.cpp"),
     os.path.join(HERE, "csrc", "kvx_events.cu"),
+    os.path.join(HERE, "csrc", "kvx_q4.cu"),
 ]
 HEADERS = [
     os.path.join(HERE, "csrc", "kvx_plan.h"),
     os.path.join(HERE, "csrc", "kvx_worklist.h"),
     os.path.join(HERE, "csrc", "kvx_kernels.cuh"),
+    os.path.join(HERE, "csrc", "kvx_q4_rows.cuh"),
+    os.path.join(HERE, "csrc", "kvx_q4_attention.cuh"),
     os.path.join(ROOT, "include", "kvx.h"),
 ]
 OUT = os.path.join(HERE, "libkvx.so")

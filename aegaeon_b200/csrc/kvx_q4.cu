@@ -1,0 +1,331 @@
+// Entry points of the 4-bit paged KV cache (include/kvx.h, kvx_q4_*): checks of
+// arguments on the host, then one or two kernel launches on the caller's stream.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "../../include/kvx.h"
+#include "kvx_q4_attention.cuh"
+#include "kvx_q4_rows.cuh"
+
+namespace kvx {
+void record_error(const std::string& msg);  // kvx_runtime.cu
+
+namespace q4 {
+namespace {
+
+int fail(int code, const std::string& msg) {
+  record_error(msg);
+  return code;
+}
+
+int cuda_fail(const char* what, cudaError_t e) {
+  return fail(KVX_ERR_CUDA, std::string(what) + ": " + cudaGetErrorName(e) + " (" +
+                                cudaGetErrorString(e) + ")");
+}
+
+bool aligned(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Geometry of a cache from the arguments of an entry point.
+int cache_of(const void* key_pages, const void* value_pages, int64_t key_stride,
+             int64_t value_stride, int64_t num_blocks, int64_t kv_heads, int64_t block_size,
+             int64_t head_dim, Cache* out) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "head_dim must be 64, 128 or 256");
+  if (block_size < 16 || block_size % 16 || block_size > 4096)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "block_size must be a multiple of 16, at most 4096");
+  if (kv_heads < 1 || kv_heads > 1024)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "kv_heads must be in [1, 1024]");
+  if (num_blocks < 0 || num_blocks > INT32_MAX)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "num_blocks must be in [0, 2^31)");
+  const int64_t head_bytes = block_size * (head_dim / 2 + 4);
+  if (num_blocks > 0) {
+    if (!key_pages || !value_pages) return fail(KVX_ERR_INVALID_ARGUMENT, "null cache pages");
+    if (!aligned(key_pages, 16) || !aligned(value_pages, 16) || key_stride % 16 ||
+        value_stride % 16)
+      return fail(KVX_ERR_INVALID_ARGUMENT,
+                  "cache pages and the strides between them must be multiples of 16 bytes");
+    if (key_stride < kv_heads * head_bytes || value_stride < kv_heads * head_bytes)
+      return fail(KVX_ERR_INVALID_ARGUMENT, "page stride below the size of a page");
+  }
+  out->pages[0] = static_cast<uint8_t*>(const_cast<void*>(key_pages));
+  out->pages[1] = static_cast<uint8_t*>(const_cast<void*>(value_pages));
+  out->stride[0] = key_stride;
+  out->stride[1] = value_stride;
+  out->num_blocks = num_blocks;
+  out->kv_heads = int(kv_heads);
+  out->block_size = int(block_size);
+  out->head_bytes = int(head_bytes);
+  return KVX_OK;
+}
+
+int64_t element_size(int dtype) { return dtype == kFp32 ? 4 : 2; }
+
+bool rows_vec(const Rows& r, int dtype) {
+  const int64_t e = element_size(dtype);
+  return aligned(r.base, 16) && r.token_stride * e % 16 == 0 && r.head_stride * e % 16 == 0;
+}
+
+template <typename T, int D>
+void launch_rows(bool write, bool vec, const RowArgs& a, unsigned grid, cudaStream_t s) {
+  if (write) {
+    if (vec) q4_write<T, D, true><<<grid, kRowThreads, 0, s>>>(a);
+    else q4_write<T, D, false><<<grid, kRowThreads, 0, s>>>(a);
+  } else {
+    if (vec) q4_read<T, D, true><<<grid, kRowThreads, 0, s>>>(a);
+    else q4_read<T, D, false><<<grid, kRowThreads, 0, s>>>(a);
+  }
+}
+
+template <typename T>
+void launch_rows(bool write, bool vec, int head_dim, const RowArgs& a, unsigned grid,
+                 cudaStream_t s) {
+  if (head_dim == 64) launch_rows<T, 64>(write, vec, a, grid, s);
+  else if (head_dim == 128) launch_rows<T, 128>(write, vec, a, grid, s);
+  else launch_rows<T, 256>(write, vec, a, grid, s);
+}
+
+int run_rows(bool write, RowArgs& a, int dtype, int64_t num_tokens, int64_t head_dim,
+             void* stream) {
+  if (dtype != kBf16 && dtype != kFp16 && dtype != kFp32)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "unknown dtype");
+  if (num_tokens < 0) return fail(KVX_ERR_INVALID_ARGUMENT, "negative token count");
+  if (num_tokens == 0) return KVX_OK;
+  if (!a.rows[0].base || !a.rows[1].base || !a.slots)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "null argument");
+  for (const Rows& r : a.rows)
+    if (!aligned(r.base, element_size(dtype)))
+      return fail(KVX_ERR_INVALID_ARGUMENT, "rows are not aligned to their type");
+  a.num_rows = num_tokens * a.cache.kv_heads;
+  const int64_t per_block = kRowThreads / (head_dim / 16);
+  const int64_t grid = (a.num_rows + per_block - 1) / per_block;
+  if (grid > INT32_MAX) return fail(KVX_ERR_INVALID_ARGUMENT, "too many tokens in one call");
+  const bool vec = rows_vec(a.rows[0], dtype) && rows_vec(a.rows[1], dtype);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == kBf16) launch_rows<__nv_bfloat16>(write, vec, int(head_dim), a, unsigned(grid), s);
+  else if (dtype == kFp16) launch_rows<__half>(write, vec, int(head_dim), a, unsigned(grid), s);
+  else launch_rows<float>(write, vec, int(head_dim), a, unsigned(grid), s);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? KVX_OK : cuda_fail(write ? "q4_write" : "q4_read", e);
+}
+
+// ---- attention -----------------------------------------------------------------
+
+// Query rows of a tile: the smallest of 8, 16, 32 that holds a sequence's rows
+// (the row count pads to it), at most 16 where D = 256 fills the registers.
+int tile_rows(int64_t rows, int64_t head_dim) {
+  if (rows <= 8) return 8;
+  if (rows <= 16 || head_dim == 256) return 16;
+  return 32;
+}
+
+// CTAs that are resident on the device at once.
+int resident(int rows, int64_t head_dim, int sms) {
+  return sms * (rows <= 16 && head_dim <= 128 ? 2 : 1);
+}
+
+int sm_count(int* sms) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
+  return e == cudaSuccess ? KVX_OK : cuda_fail("cudaDeviceGetAttribute", e);
+}
+
+uint64_t workspace_of(int rows, int64_t head_dim, int sms) {
+  return 2ull * resident(rows, head_dim, sms) * rows * (4 * head_dim + 8);
+}
+
+template <typename T, int D, int NT>
+int launch_attention(const AttnArgs& a, int grid, cudaStream_t s) {
+  constexpr int shared = Shape<D>::kShared;
+  cudaError_t e = cudaFuncSetAttribute(q4_attend<T, D, NT>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+  if (e != cudaSuccess) return cuda_fail("cudaFuncSetAttribute", e);
+  q4_attend<T, D, NT><<<grid, kThreads, shared, s>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail("q4_attend", e);
+  if (grid == 1) return KVX_OK;  // one CTA has the whole of every item
+  // The join's launch and its search for its item overlap the attention.
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(grid - 1));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, q4_join<T, D, NT>, a, grid);
+  return e == cudaSuccess ? KVX_OK : cuda_fail("q4_join", e);
+}
+
+template <typename T>
+int launch_attention(const AttnArgs& a, int64_t head_dim, int rows, int grid, cudaStream_t s) {
+  if (head_dim == 64) {
+    if (rows == 8) return launch_attention<T, 64, 1>(a, grid, s);
+    if (rows == 16) return launch_attention<T, 64, 2>(a, grid, s);
+    return launch_attention<T, 64, 4>(a, grid, s);
+  }
+  if (head_dim == 128) {
+    if (rows == 8) return launch_attention<T, 128, 1>(a, grid, s);
+    if (rows == 16) return launch_attention<T, 128, 2>(a, grid, s);
+    return launch_attention<T, 128, 4>(a, grid, s);
+  }
+  if (rows == 8) return launch_attention<T, 256, 1>(a, grid, s);
+  return launch_attention<T, 256, 2>(a, grid, s);
+}
+
+}  // namespace
+
+// The device status word of this part (kvx_device_status reads all of them).
+int q4_device_status(int reset, int* value) {
+  cudaError_t e = cudaMemcpyFromSymbol(value, g_q4_status, sizeof(int));
+  if (e == cudaSuccess && reset && *value) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_q4_status, &zero, sizeof(int));
+  }
+  return e == cudaSuccess ? KVX_OK : cuda_fail("q4 status", e);
+}
+
+}  // namespace q4
+}  // namespace kvx
+
+using namespace kvx;
+using namespace kvx::q4;
+
+extern "C" {
+
+int kvx_q4_write(const void* key, const void* value, int dtype, int64_t num_tokens,
+                 int64_t key_token_stride, int64_t key_head_stride, int64_t value_token_stride,
+                 int64_t value_head_stride, const int64_t* slots, void* key_pages,
+                 void* value_pages, int64_t key_page_stride, int64_t value_page_stride,
+                 int64_t num_blocks, int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                 void* stream) {
+  record_error("");
+  RowArgs a{};
+  int rc = cache_of(key_pages, value_pages, key_page_stride, value_page_stride, num_blocks,
+                    kv_heads, block_size, head_dim, &a.cache);
+  if (rc) return rc;
+  a.rows[0] = Rows{const_cast<void*>(key), key_token_stride, key_head_stride};
+  a.rows[1] = Rows{const_cast<void*>(value), value_token_stride, value_head_stride};
+  a.slots = slots;
+  return run_rows(true, a, dtype, num_tokens, head_dim, stream);
+}
+
+int kvx_q4_read(const void* key_pages, const void* value_pages, int64_t key_page_stride,
+                int64_t value_page_stride, int64_t num_blocks, int64_t kv_heads,
+                int64_t block_size, int64_t head_dim, const int64_t* slots, int64_t num_tokens,
+                void* key, void* value, int dtype, int64_t key_token_stride,
+                int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
+                void* stream) {
+  record_error("");
+  RowArgs a{};
+  int rc = cache_of(key_pages, value_pages, key_page_stride, value_page_stride, num_blocks,
+                    kv_heads, block_size, head_dim, &a.cache);
+  if (rc) return rc;
+  a.rows[0] = Rows{key, key_token_stride, key_head_stride};
+  a.rows[1] = Rows{value, value_token_stride, value_head_stride};
+  a.slots = slots;
+  return run_rows(false, a, dtype, num_tokens, head_dim, stream);
+}
+
+int kvx_q4_attention_workspace(int64_t head_dim, int64_t rows_per_sequence, uint64_t* bytes_out) {
+  record_error("");
+  if (!bytes_out) return fail(KVX_ERR_INVALID_ARGUMENT, "null bytes_out");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "head_dim must be 64, 128 or 256");
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc) return rc;
+  *bytes_out = workspace_of(tile_rows(rows_per_sequence, head_dim), head_dim, sms);
+  return KVX_OK;
+}
+
+int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t query_head_stride,
+                     void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                     int dtype, int64_t num_tokens, int64_t num_heads, const void* key_pages,
+                     const void* value_pages, int64_t key_page_stride, int64_t value_page_stride,
+                     int64_t num_blocks, int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                     const int32_t* block_tables, int64_t table_stride, int64_t table_width,
+                     const int32_t* seq_lens, const int32_t* query_starts, int64_t batch,
+                     double scale, int64_t window, int64_t sinks, void* workspace,
+                     uint64_t workspace_bytes, void* stream) {
+  record_error("");
+  AttnArgs a{};
+  int rc = cache_of(key_pages, value_pages, key_page_stride, value_page_stride, num_blocks,
+                    kv_heads, block_size, head_dim, &a.cache);
+  if (rc) return rc;
+  if (dtype != kBf16 && dtype != kFp16)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "queries must be bf16 or fp16");
+  if (num_tokens < 0 || batch < 0 || table_width < 0)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "negative count");
+  if (num_heads < 1 || num_heads % kv_heads)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "query heads must be a multiple of kv_heads");
+  if (window < 0 || sinks < 0)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "window and sinks must not be negative");
+  if (!std::isfinite(scale)) return fail(KVX_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (num_tokens == 0 || batch == 0) return KVX_OK;
+  if (!query || !out || !seq_lens || (!block_tables && table_width > 0))
+    return fail(KVX_ERR_INVALID_ARGUMENT, "null argument");
+  if (!aligned(query, 2) || !aligned(out, 2) || !aligned(workspace, 16))
+    return fail(KVX_ERR_INVALID_ARGUMENT, "an argument is not aligned to its type");
+  const int64_t group = num_heads / kv_heads;
+  if (!query_starts && num_tokens % batch)
+    return fail(KVX_ERR_LENGTH_MISMATCH,
+                "without query_starts every sequence has the same number of query tokens");
+  if (num_tokens * group >= (1ll << 30) || batch >= (1ll << 30) ||
+      table_width * block_size >= (1ll << 30))
+    return fail(KVX_ERR_INVALID_ARGUMENT, "request too large for one call");
+  const int64_t queries = query_starts ? num_tokens : num_tokens / batch;
+  const int rows = tile_rows(queries * group, head_dim);
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc) return rc;
+  if (!workspace || workspace_bytes < workspace_of(rows, head_dim, sms))
+    return fail(KVX_ERR_INVALID_ARGUMENT,
+                "workspace smaller than kvx_q4_attention_workspace() says");
+  a.query = query;
+  a.q_token = query_token_stride;
+  a.q_head = query_head_stride;
+  a.q_vec = aligned(query, 16) && query_token_stride % 8 == 0 && query_head_stride % 8 == 0;
+  a.out = out;
+  a.o_token = out_token_stride;
+  a.o_head = out_head_stride;
+  a.o_vec = aligned(out, 8) && out_token_stride % 4 == 0 && out_head_stride % 4 == 0;
+  a.lse = lse;
+  a.tables = block_tables;
+  a.table_stride = table_stride;
+  a.table_width = int(table_width);
+  a.lens = seq_lens;
+  a.starts = query_starts;
+  a.batch = int(batch);
+  a.queries = int(queries);
+  a.num_tokens = int(num_tokens);
+  a.group = int(group);
+  a.scale_log2 = float(scale * 1.4426950408889634);
+  a.window = window == 0 || window > kNoWindow ? kNoWindow : int(window);
+  a.sinks = a.window == kNoWindow ? 0 : int(std::min<int64_t>(sinks, kNoWindow));
+  a.upp = int(block_size / 16);
+  a.upp_shift = -1;
+  for (int i = 0; i < 9; ++i)
+    if (a.upp == 1 << i) a.upp_shift = i;
+  // Shares: the CTAs that are resident at once, or fewer where even the longest
+  // sequences that the tables can hold give them less than kMinUnits each.
+  const int64_t tiles = query_starts ? num_tokens * group / rows + batch
+                                     : batch * ((queries * group + rows - 1) / rows);
+  const int64_t units = std::max<int64_t>(table_width * a.upp, 1);
+  int64_t grid = resident(rows, head_dim, sms);
+  const double bound = double(tiles) * double(kv_heads) * double(units) / kMinUnits;
+  if (bound < double(grid)) grid = std::max<int64_t>(1, int64_t(std::ceil(bound)));
+  const int64_t pieces = 2ll * resident(rows, head_dim, sms) * rows;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * head_dim);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == kBf16 ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), s)
+                        : launch_attention<__half>(a, head_dim, rows, int(grid), s);
+}
+
+}  // extern "C"

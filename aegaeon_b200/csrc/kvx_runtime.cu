@@ -33,6 +33,10 @@
 #include "kvx_plan.h"
 
 namespace kvx {
+namespace q4 {
+int q4_device_status(int reset, int* value);  // kvx_q4.cu
+}
+
 namespace {
 
 thread_local std::string t_last_error;
@@ -1885,6 +1889,10 @@ int kvx_device_status(int device, int reset, int* status_out) {
     const int zero = 0;
     KVX_CUDA(cudaMemcpyToSymbol(g_kvx_device_status, &zero, sizeof(int)));
   }
+  int q4_word = 0;
+  const int rc = q4::q4_device_status(reset, &q4_word);
+  if (rc) return rc;
+  if (v == 0) v = q4_word;
   *status_out = v;
   return KVX_OK;
 }

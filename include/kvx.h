@@ -261,7 +261,8 @@ int kvx_plan_swap(const int64_t* source_block_ids,
  * kvx_last_mode: the transfer mode the last successful copy call of this
  * thread used (KVX_MODE_SM / _CE / _SM_BULK / _CE_EXTENT).
  * kvx_device_status: reads (and with reset != 0 clears) the device error word
- * written by kernels whose bounded waits gave up; synchronizes the device.  */
+ * written by kernels whose bounded waits gave up, or by a kvx_q4_* kernel that
+ * met an id or length outside its buffer; synchronizes the device.            */
 int kvx_last_mode(void);
 /* Number of copy kernels this process has launched through the library. */
 uint64_t kvx_kernel_launches(void);
@@ -343,6 +344,85 @@ int kvx_set_option(const char* name, int64_t value);
  * Replaces: read_safetensors_meta_as_json, quick_model_loader/rsrc/lib.rs:19-51. */
 int kvx_safetensors_meta_json(const char* file_path, char* out,
                               uint64_t capacity, uint64_t* length_out);
+
+/* ---- 4-bit paged KV cache ---------------------------------------------------
+ * No counterpart in the reference (its caches hold 16-bit values).  One tensor
+ * (K or V) of a layer is kept as pages of one block each, kv heads outermost:
+ *   [kv_heads][ block_size * head_dim/2 bytes of codes,
+ *               block_size * (fp16 scale, fp16 zero) ]
+ * A value is scale * code + zero, with one scale and zero for each token and
+ * head.  The codes of a token are head_dim/2 consecutive bytes, the even
+ * dimension in the low nibble.  A page is plain bytes: kvx_swap,
+ * kvx_swap_blocks and kvx_migrate_blocks move it as they move any page.
+ *
+ * Common arguments: key_pages / value_pages: page 0 of the two tensors, device
+ * memory of the current device, 16-byte aligned; *_page_stride: bytes from one
+ * page to the next (a multiple of 16, at least one page); num_blocks pages in
+ * each; block_size a multiple of 16 (at most 4096); head_dim 64, 128 or 256.
+ * dtype: KVX_DTYPE_*.  Strides of rows are in elements; the elements of one
+ * row are contiguous.  Slot s is token s % block_size of block s / block_size.
+ * All device pointers; nothing is read back: a slot, block id or length that
+ * is outside its buffer is skipped by the kernels and reported by
+ * kvx_device_status (KVX_ERR_BLOCK_ID, KVX_ERR_EXTENT).  Every call may be
+ * captured into a CUDA graph.
+ *
+ * kvx_q4_write: quantises key and value [num_tokens][kv_heads][head_dim] into
+ * slots[i] of token i (negative: the row is skipped, as padding is).  With x a
+ * row in 32 bits, clamped to the finite range of fp16:
+ *   scale = fp16((max - min) / 15), zero = fp16(min),
+ *   code = rint((x - zero) / scale) in [0, 15], ties to even, 0 if scale is 0.
+ * A row with a NaN or an infinity is stored as NaN.  The slots of one call are
+ * distinct; what a repeated slot holds afterwards is unspecified.
+ *
+ * kvx_q4_read: gives the rows of slots[i] back into key and value (rounded
+ * once from 32 bits); zeros for a negative slot.
+ *
+ * kvx_q4_attention: causal attention of query [num_tokens][num_heads][head_dim]
+ * over the cache.  Sequence b has seq_lens[b] tokens in the blocks
+ * block_tables[b * table_stride + 0 ...] (table_width entries); its query
+ * tokens are the last ones of them: rows [query_starts[b], query_starts[b+1])
+ * of query, or num_tokens / batch each when query_starts is NULL.  Query head
+ * h reads kv head h / (num_heads / kv_heads).  A query at position p sees the
+ * tokens j <= p, with window > 0 only those with j > p - window or j < sinks.
+ * out: softmax(scale * q k) v, lse (optional, [num_tokens][num_heads]): the
+ * natural log-sum-exp of the scores.  A row that sees nothing gives 0 and
+ * -inf.  Rows behind the last sequence are left as they were.  workspace:
+ * kvx_q4_attention_workspace() bytes, 16-byte aligned, for this call alone
+ * until it has finished; rows_per_sequence is the call's num_tokens (divided
+ * by batch without query_starts) * num_heads / kv_heads.                       */
+#define KVX_DTYPE_BF16 0
+#define KVX_DTYPE_FP16 1
+#define KVX_DTYPE_FP32 2
+int kvx_q4_write(const void* key, const void* value, int dtype,
+                 int64_t num_tokens, int64_t key_token_stride,
+                 int64_t key_head_stride, int64_t value_token_stride,
+                 int64_t value_head_stride, const int64_t* slots,
+                 void* key_pages, void* value_pages, int64_t key_page_stride,
+                 int64_t value_page_stride, int64_t num_blocks,
+                 int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                 void* stream);
+int kvx_q4_read(const void* key_pages, const void* value_pages,
+                int64_t key_page_stride, int64_t value_page_stride,
+                int64_t num_blocks, int64_t kv_heads, int64_t block_size,
+                int64_t head_dim, const int64_t* slots, int64_t num_tokens,
+                void* key, void* value, int dtype, int64_t key_token_stride,
+                int64_t key_head_stride, int64_t value_token_stride,
+                int64_t value_head_stride, void* stream);
+int kvx_q4_attention_workspace(int64_t head_dim, int64_t rows_per_sequence,
+                               uint64_t* bytes_out);
+int kvx_q4_attention(const void* query, int64_t query_token_stride,
+                     int64_t query_head_stride, void* out,
+                     int64_t out_token_stride, int64_t out_head_stride,
+                     float* lse, int dtype, int64_t num_tokens,
+                     int64_t num_heads, const void* key_pages,
+                     const void* value_pages, int64_t key_page_stride,
+                     int64_t value_page_stride, int64_t num_blocks,
+                     int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                     const int32_t* block_tables, int64_t table_stride,
+                     int64_t table_width, const int32_t* seq_lens,
+                     const int32_t* query_starts, int64_t batch, double scale,
+                     int64_t window, int64_t sinks, void* workspace,
+                     uint64_t workspace_bytes, void* stream);
 
 /* ---- allocation-free swap ---------------------------------------------------
  * No counterpart in the reference.  For callers that must not allocate GPU
