@@ -107,13 +107,13 @@ SIGNATURES = {
     "kvx_configure": (_int, [_i64, _i64, _i64, _i64, _i64]),
     "kvx_set_option": (_int, [ctypes.c_char_p, _i64]),
     "kvx_swap_noalloc": (_int, [_p_i64, _p_i64, _i64, _int, _vp, _u64, _u64, _vp, _u64, _vp]),
-    "kvx_q4_write": (_int, [_vp, _vp, _int] + [_i64] * 5 + [_vp] * 3 + [_i64] * 6 + [_vp]),
-    "kvx_q4_read": (_int, [_vp, _vp] + [_i64] * 6 + [_vp, _i64, _vp, _vp, _int] + [_i64] * 4
+    "kvx_q4_write": (_int, [_vp, _vp, _int] + [_i64] * 5 + [_vp] * 3 + [_i64] * 5 + [_vp]),
+    "kvx_q4_read": (_int, [_vp, _vp] + [_i64] * 5 + [_vp, _i64, _vp, _vp, _int] + [_i64] * 4
                     + [_vp]),
     "kvx_q4_attention_workspace": (_int, [_i64, _i64, _p_u64]),
     "kvx_q4_attention": (
         _int,
-        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _int, _i64, _i64, _vp, _vp] + [_i64] * 6
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _int, _i64, _i64, _vp, _vp] + [_i64] * 5
         + [_vp, _i64, _i64, _vp, _vp, _i64, ctypes.c_double, _i64, _i64, _vp, _u64, _vp],
     ),
     "kvx_safetensors_meta_json": (_int, [ctypes.c_char_p, ctypes.c_char_p, _u64, _p_u64]),

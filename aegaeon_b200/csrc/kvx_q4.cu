@@ -30,8 +30,7 @@ int cuda_fail(const char* what, cudaError_t e) {
 bool aligned(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // Geometry of a cache from the arguments of an entry point.
-int cache_of(const void* key_pages, const void* value_pages, int64_t key_stride,
-             int64_t value_stride, int64_t num_blocks, int64_t kv_heads, int64_t block_size,
+int cache_of(const void* key_pages, const void* value_pages, int64_t stride, int64_t num_blocks, int64_t kv_heads, int64_t block_size,
              int64_t head_dim, Cache* out) {
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return fail(KVX_ERR_INVALID_ARGUMENT, "head_dim must be 64, 128 or 256");
@@ -44,17 +43,15 @@ int cache_of(const void* key_pages, const void* value_pages, int64_t key_stride,
   const int64_t head_bytes = block_size * (head_dim / 2 + 4);
   if (num_blocks > 0) {
     if (!key_pages || !value_pages) return fail(KVX_ERR_INVALID_ARGUMENT, "null cache pages");
-    if (!aligned(key_pages, 16) || !aligned(value_pages, 16) || key_stride % 16 ||
-        value_stride % 16)
+    if (!aligned(key_pages, 16) || !aligned(value_pages, 16) || stride % 16)
       return fail(KVX_ERR_INVALID_ARGUMENT,
-                  "cache pages and the strides between them must be multiples of 16 bytes");
-    if (key_stride < kv_heads * head_bytes || value_stride < kv_heads * head_bytes)
+                  "cache pages and the stride between them must be multiples of 16 bytes");
+    if (stride < kv_heads * head_bytes)
       return fail(KVX_ERR_INVALID_ARGUMENT, "page stride below the size of a page");
   }
   out->pages[0] = static_cast<uint8_t*>(const_cast<void*>(key_pages));
   out->pages[1] = static_cast<uint8_t*>(const_cast<void*>(value_pages));
-  out->stride[0] = key_stride;
-  out->stride[1] = value_stride;
+  out->stride = stride;
   out->num_blocks = num_blocks;
   out->kv_heads = int(kv_heads);
   out->block_size = int(block_size);
@@ -134,12 +131,16 @@ int sm_count(int* sms) {
   return e == cudaSuccess ? KVX_OK : cuda_fail("cudaDeviceGetAttribute", e);
 }
 
+// Items up to which the join takes a block for each row: a few dozen CTAs then
+// share an item, and the rows' blocks still fit the device at once.
+constexpr int64_t kJoinByRow = 64;
+
 uint64_t workspace_of(int rows, int64_t head_dim, int sms) {
   return 2ull * resident(rows, head_dim, sms) * rows * (4 * head_dim + 8);
 }
 
 template <typename T, int D, int NT>
-int launch_attention(const AttnArgs& a, int grid, cudaStream_t s) {
+int launch_attention(const AttnArgs& a, int grid, int64_t items, cudaStream_t s) {
   constexpr int shared = Shape<D>::kShared;
   cudaError_t e = cudaFuncSetAttribute(q4_attend<T, D, NT>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
@@ -149,33 +150,38 @@ int launch_attention(const AttnArgs& a, int grid, cudaStream_t s) {
   if (e != cudaSuccess) return cuda_fail("q4_attend", e);
   if (grid == 1) return KVX_OK;  // one CTA has the whole of every item
   // The join's launch and its search for its item overlap the attention.
+  // A block for each row where there are fewer items than a warp would have
+  // pieces to walk through, otherwise one for each border between shares.
+  const bool by_row = items <= kJoinByRow;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(grid - 1));
+  cfg.gridDim = dim3(by_row ? unsigned(items * 8 * NT) : unsigned(grid - 1));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, q4_join<T, D, NT>, a, grid);
+  e = by_row ? cudaLaunchKernelEx(&cfg, q4_join<T, D, NT, true>, a, grid)
+             : cudaLaunchKernelEx(&cfg, q4_join<T, D, NT, false>, a, grid);
   return e == cudaSuccess ? KVX_OK : cuda_fail("q4_join", e);
 }
 
 template <typename T>
-int launch_attention(const AttnArgs& a, int64_t head_dim, int rows, int grid, cudaStream_t s) {
+int launch_attention(const AttnArgs& a, int64_t head_dim, int rows, int grid, int64_t items,
+                     cudaStream_t s) {
   if (head_dim == 64) {
-    if (rows == 8) return launch_attention<T, 64, 1>(a, grid, s);
-    if (rows == 16) return launch_attention<T, 64, 2>(a, grid, s);
-    return launch_attention<T, 64, 4>(a, grid, s);
+    if (rows == 8) return launch_attention<T, 64, 1>(a, grid, items, s);
+    if (rows == 16) return launch_attention<T, 64, 2>(a, grid, items, s);
+    return launch_attention<T, 64, 4>(a, grid, items, s);
   }
   if (head_dim == 128) {
-    if (rows == 8) return launch_attention<T, 128, 1>(a, grid, s);
-    if (rows == 16) return launch_attention<T, 128, 2>(a, grid, s);
-    return launch_attention<T, 128, 4>(a, grid, s);
+    if (rows == 8) return launch_attention<T, 128, 1>(a, grid, items, s);
+    if (rows == 16) return launch_attention<T, 128, 2>(a, grid, items, s);
+    return launch_attention<T, 128, 4>(a, grid, items, s);
   }
-  if (rows == 8) return launch_attention<T, 256, 1>(a, grid, s);
-  return launch_attention<T, 256, 2>(a, grid, s);
+  if (rows == 8) return launch_attention<T, 256, 1>(a, grid, items, s);
+  return launch_attention<T, 256, 2>(a, grid, items, s);
 }
 
 }  // namespace
@@ -201,13 +207,12 @@ extern "C" {
 int kvx_q4_write(const void* key, const void* value, int dtype, int64_t num_tokens,
                  int64_t key_token_stride, int64_t key_head_stride, int64_t value_token_stride,
                  int64_t value_head_stride, const int64_t* slots, void* key_pages,
-                 void* value_pages, int64_t key_page_stride, int64_t value_page_stride,
-                 int64_t num_blocks, int64_t kv_heads, int64_t block_size, int64_t head_dim,
-                 void* stream) {
+                 void* value_pages, int64_t page_stride, int64_t num_blocks, int64_t kv_heads,
+                 int64_t block_size, int64_t head_dim, void* stream) {
   record_error("");
   RowArgs a{};
-  int rc = cache_of(key_pages, value_pages, key_page_stride, value_page_stride, num_blocks,
-                    kv_heads, block_size, head_dim, &a.cache);
+  int rc = cache_of(key_pages, value_pages, page_stride, num_blocks, kv_heads, block_size,
+                    head_dim, &a.cache);
   if (rc) return rc;
   a.rows[0] = Rows{const_cast<void*>(key), key_token_stride, key_head_stride};
   a.rows[1] = Rows{const_cast<void*>(value), value_token_stride, value_head_stride};
@@ -215,16 +220,16 @@ int kvx_q4_write(const void* key, const void* value, int dtype, int64_t num_toke
   return run_rows(true, a, dtype, num_tokens, head_dim, stream);
 }
 
-int kvx_q4_read(const void* key_pages, const void* value_pages, int64_t key_page_stride,
-                int64_t value_page_stride, int64_t num_blocks, int64_t kv_heads,
-                int64_t block_size, int64_t head_dim, const int64_t* slots, int64_t num_tokens,
+int kvx_q4_read(const void* key_pages, const void* value_pages, int64_t page_stride,
+                int64_t num_blocks, int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                const int64_t* slots, int64_t num_tokens,
                 void* key, void* value, int dtype, int64_t key_token_stride,
                 int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
                 void* stream) {
   record_error("");
   RowArgs a{};
-  int rc = cache_of(key_pages, value_pages, key_page_stride, value_page_stride, num_blocks,
-                    kv_heads, block_size, head_dim, &a.cache);
+  int rc = cache_of(key_pages, value_pages, page_stride, num_blocks, kv_heads, block_size,
+                    head_dim, &a.cache);
   if (rc) return rc;
   a.rows[0] = Rows{key, key_token_stride, key_head_stride};
   a.rows[1] = Rows{value, value_token_stride, value_head_stride};
@@ -247,16 +252,15 @@ int kvx_q4_attention_workspace(int64_t head_dim, int64_t rows_per_sequence, uint
 int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t query_head_stride,
                      void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
                      int dtype, int64_t num_tokens, int64_t num_heads, const void* key_pages,
-                     const void* value_pages, int64_t key_page_stride, int64_t value_page_stride,
-                     int64_t num_blocks, int64_t kv_heads, int64_t block_size, int64_t head_dim,
-                     const int32_t* block_tables, int64_t table_stride, int64_t table_width,
+                     const void* value_pages, int64_t page_stride, int64_t num_blocks,
+                     int64_t kv_heads, int64_t block_size, int64_t head_dim, const int32_t* block_tables, int64_t table_stride, int64_t table_width,
                      const int32_t* seq_lens, const int32_t* query_starts, int64_t batch,
                      double scale, int64_t window, int64_t sinks, void* workspace,
                      uint64_t workspace_bytes, void* stream) {
   record_error("");
   AttnArgs a{};
-  int rc = cache_of(key_pages, value_pages, key_page_stride, value_page_stride, num_blocks,
-                    kv_heads, block_size, head_dim, &a.cache);
+  int rc = cache_of(key_pages, value_pages, page_stride, num_blocks, kv_heads, block_size,
+                    head_dim, &a.cache);
   if (rc) return rc;
   if (dtype != kBf16 && dtype != kFp16)
     return fail(KVX_ERR_INVALID_ARGUMENT, "queries must be bf16 or fp16");
@@ -305,7 +309,8 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   a.queries = int(queries);
   a.num_tokens = int(num_tokens);
   a.group = int(group);
-  a.scale_log2 = float(scale * 1.4426950408889634);
+  a.scale_log2 = float(std::fabs(scale) * 1.4426950408889634);
+  a.sign = scale < 0 ? -1.f : 1.f;
   a.window = window == 0 || window > kNoWindow ? kNoWindow : int(window);
   a.sinks = a.window == kNoWindow ? 0 : int(std::min<int64_t>(sinks, kNoWindow));
   a.upp = int(block_size / 16);
@@ -318,14 +323,16 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
                                      : batch * ((queries * group + rows - 1) / rows);
   const int64_t units = std::max<int64_t>(table_width * a.upp, 1);
   int64_t grid = resident(rows, head_dim, sms);
-  const double bound = double(tiles) * double(kv_heads) * double(units) / kMinUnits;
+  const int64_t items = tiles * kv_heads;
+  const double bound =
+      double(items) * double(units + kItemUnits) / double(kMinUnits + kItemUnits);
   if (bound < double(grid)) grid = std::max<int64_t>(1, int64_t(std::ceil(bound)));
   const int64_t pieces = 2ll * resident(rows, head_dim, sms) * rows;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == kBf16 ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), s)
-                        : launch_attention<__half>(a, head_dim, rows, int(grid), s);
+  return dtype == kBf16 ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), items, s)
+                        : launch_attention<__half>(a, head_dim, rows, int(grid), items, s);
 }
 
 }  // extern "C"

@@ -26,6 +26,9 @@ constexpr int kNoWindow = 1 << 30;
 // Fewest 16-token units a CTA takes: two for each warp.  Fewer make the join
 // the larger part of the work.
 constexpr int kMinUnits = 2 * kWarps;
+// What an item (a tile of query rows with one kv head) costs besides its units,
+// in units: its queries, its first block ids and the join of the warps.
+constexpr int kItemUnits = 16;
 
 struct AttnArgs {
   Cache cache;
@@ -43,7 +46,8 @@ struct AttnArgs {
   int queries;
   int num_tokens;
   int group;                // query heads of a kv head
-  float scale_log2;         // softmax scale * log2(e)
+  float scale_log2;         // |softmax scale| * log2(e)
+  float sign;               // of the softmax scale
   int window;               // kNoWindow: none
   int sinks;                // 0 without a window
   int upp;                  // 16-token units of a page
@@ -96,58 +100,47 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Seq& s, int row
   return v;
 }
 
-// Sum of f(0..n-1) over the block, and the place of `pos` in its running sum.
-template <class F>
-__device__ int64_t block_total(F f, int n, int64_t* sm) {
-  int64_t v = 0;
-  for (int i = threadIdx.x; i < n; i += kThreads) v += f(i);
-#pragma unroll
-  for (int d = 16; d; d /= 2) v += __shfl_xor_sync(~0u, v, d);
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) v += sm[i];
-  __syncthreads();
-  return v;
-}
-
+// Work of all sequences, and the place of a position in its running sum.  Every
+// thread takes a run of sequences; `at` maps the total to the position.
 struct Place {
-  int index;       // the i whose part holds the position, n when none does
-  int64_t before;  // sum of f(0..index-1)
+  int index;       // the sequence whose part holds the position, n when none does
+  int64_t before;  // work of the sequences before it
 };
 
-template <class F>
-__device__ Place block_locate(F f, int n, int64_t pos, int64_t* sm, Place* found) {
+template <class F, class G>
+__device__ __forceinline__ int64_t block_locate(F f, int n, G at, int64_t* sm, Place* found,
+                                                Place* place) {
+  const int run = (n + kThreads - 1) / kThreads, first = threadIdx.x * run;
+  const int last = min(first + run, n);
+  int64_t own = 0;
+  for (int i = first; i < last; ++i) own += f(i);
+  int64_t v = own;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int64_t u = __shfl_up_sync(~0u, v, d);
+    if (threadIdx.x % 32 >= d) v += u;
+  }
+  if (threadIdx.x % 32 == 31) sm[threadIdx.x / 32] = v;
   if (threadIdx.x == 0) *found = Place{n, 0};
-  int64_t base = 0;
-  for (int at = 0; at < n; at += kThreads) {
-    const int i = at + threadIdx.x;
-    const int64_t own = i < n ? f(i) : 0;
-    int64_t v = own;
+  __syncthreads();
+  int64_t before = v - own, total = 0;
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int64_t u = __shfl_up_sync(~0u, v, d);
-      if (threadIdx.x % 32 >= d) v += u;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < int(threadIdx.x / 32)) before += sm[w];
+    total += sm[w];
+  }
+  const int64_t pos = at(total);
+  if (pos >= before && pos < before + own) {
+    int i = first;
+    for (int64_t c = run > 1 ? f(i) : own; pos >= before + c; c = f(i)) {
+      before += c;
+      ++i;
     }
-    __syncthreads();
-    if (threadIdx.x % 32 == 31) sm[threadIdx.x / 32] = v;
-    __syncthreads();
-    int64_t before = base, all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < int(threadIdx.x / 32)) before += sm[w];
-      all += sm[w];
-    }
-    before += v - own;
-    if (pos >= before && pos < before + own) *found = Place{i, before};
-    base += all;
+    *found = Place{i, before};
   }
   __syncthreads();
-  const Place p = *found;
-  __syncthreads();
-  return p;
+  *place = *found;
+  return total;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -170,8 +163,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return r;
 }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
-  const int n = real ? 16 : 0;  // 0: nothing is read, 16 zero bytes are written
+// 16 bytes to shared memory; n = 0: nothing is read, zeros are written.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int n) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
                : "memory");
 }
@@ -203,8 +196,8 @@ __device__ __forceinline__ int key_dim(int j, int w) {
 template <int D, int NT>
 struct TileShared {
   uint2 q[NT][D / 16][32];  // B fragments of the queries, as mma reads them
-  float factor[NT * 8];     // scale * log2(e) and the powers of two taken out
-  float sum[NT * 8];        // sum(q) * scale * log2(e)
+  float factor[NT * 8];     // |scale| * log2(e) and the powers of two taken out
+  float sum[NT * 8];        // sum(q) in the unit of the products with the codes
   int pos[NT * 8];          // position in the sequence, -1 for rows that are none
   float m[kWarps][NT * 8];
   float l[kWarps][NT * 8];
@@ -250,17 +243,15 @@ __device__ __forceinline__ void load_queries(const AttnArgs& a, const Seq& s, in
     for (int i = 0; i < 8; ++i) {
       x[w][i] = to_float(v[i]);
       top = fmaxf(top, fabsf(x[w][i]));
-      sum += x[w][i];
     }
   }
 #pragma unroll
-  for (int d = 1; d < 4; d *= 2) {
-    top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    sum += __shfl_xor_sync(~0u, sum, d);
-  }
+  for (int d = 1; d < 4; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
   // 2^(14 - exponent of top); bounded so that both it and its inverse are normal.
   const int e = min(max(int(__float_as_uint(top) >> 23), 20), 250);
-  const float up = top > 0.f ? __uint_as_float(uint32_t(min(127 + 14 + 127 - e, 240)) << 23) : 1.f;
+  float up = top > 0.f ? __uint_as_float(uint32_t(min(127 + 14 + 127 - e, 240)) << 23) : 1.f;
+  const float factor = a.scale_log2 * 16777216.f / up;
+  up *= a.sign;
 #pragma unroll
   for (int w = 0; w < kW; ++w) {
     uint32_t f[4];
@@ -268,14 +259,17 @@ __device__ __forceinline__ void load_queries(const AttnArgs& a, const Seq& s, in
     for (int i = 0; i < 4; ++i) {
       const float u = (i % 2) ? up * 0.0625f : up;  // odd nibbles are 16 times as large
       const __half2 h = __floats2half2_rn(x[w][i] * u, x[w][i + 4] * u);
+      sum += x[w][i] * up + x[w][i + 4] * up;
       __builtin_memcpy(&f[i], &h, 4);
     }
     sh.q[warp][2 * w][lane] = make_uint2(f[0], f[1]);
     sh.q[warp][2 * w + 1][lane] = make_uint2(f[2], f[3]);
   }
+#pragma unroll
+  for (int d = 1; d < 4; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
   if (j == 0) {
-    sh.factor[r] = a.scale_log2 * 16777216.f / up;
-    sh.sum[r] = a.scale_log2 * sum;
+    sh.factor[r] = fmaxf(factor, 1e-37f);  // never 0: hidden scores are -inf
+    sh.sum[r] = sum * 5.9604644775390625e-8f;
     sh.pos[r] = pos;
   }
 }
@@ -285,100 +279,227 @@ template <int D, int NT>
 struct WarpState {
   float o[NT][D / 16][4];  // sum of p * s * C * code, dimensions as in value_dim()
   float ps[NT][4];         // sum of the same weights as the matrix instruction saw them
-  float m[NT][2], l[NT][2], z[NT][2];
+  float2 m[NT], l[NT];     // reference point and sum of the weights, by column
+  float z[NT][2];          // sum of p * (zero + 7.5 scale)
   float c;                 // C: power of two on the V scales, so that weights suit fp16
 };
 
-// AB units at a time: scores, softmax, products.  `first` is the first unit's
-// number in the sequence, -1 for a unit that is not there.
-template <int D, int NT, int AB, bool kMasked>
-__device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared<D, NT>& sh,
-                                             const uint2* qreg, const uint8_t* stage,
-                                             int unit0, const int (&number)[AB],
-                                             const float (&factor)[NT][2],
-                                             const float (&qsum)[NT][2], const int (&pos)[NT][2],
-                                             const Span& v, WarpState<D, NT>& st) {
-  const int lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
-  constexpr int kKW = Shape<D>::kKeyWords, kVW = Shape<D>::kValueWords, kUnit = Shape<D>::kUnit;
-  const uint8_t* keys = stage;
-  const uint8_t* values = stage + 2 * kUnit;
-  const uint8_t* params = stage + 4 * kUnit;
-  float x[AB][NT][4];
-#pragma unroll
-  for (int u = 0; u < AB; ++u) {
-    uint32_t kw[2][kKW];
-    const uint8_t* unit = keys + (unit0 + u) * kUnit;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const uint8_t* row = unit + (g + 8 * r) * (D / 2);
-      if constexpr (D == 64) {
-        const uint2 v = *reinterpret_cast<const uint2*>(row + 8 * j);
-        kw[r][0] = v.x, kw[r][1] = v.y;
-      } else if constexpr (D == 128) {
-        const uint4 v = *reinterpret_cast<const uint4*>(row + 16 * j);
-        kw[r][0] = v.x, kw[r][1] = v.y, kw[r][2] = v.z, kw[r][3] = v.w;
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 v = *reinterpret_cast<const uint4*>(row + 16 * ((4 * h + j) ^ (4 * (g & 1))));
-          kw[r][4 * h] = v.x, kw[r][4 * h + 1] = v.y, kw[r][4 * h + 2] = v.z, kw[r][4 * h + 3] = v.w;
-        }
-      }
+template <int kOffset>
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a), "n"(kOffset));
+  return v;
+}
+template <int kOffset>
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2+%3];" : "=r"(v.x), "=r"(v.y) : "r"(a), "n"(kOffset));
+  return v;
+}
+template <int kOffset>
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(v) : "r"(a), "n"(kOffset));
+  return v;
+}
+__device__ __forceinline__ float2 half2_at(uint32_t x) {
+  __half2 h;
+  __builtin_memcpy(&h, &x, 4);
+  return __half22float2(h);
+}
+// Two additions, or two fused multiply-adds, in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{.reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+// Shared-memory addresses of a lane's parts of a stage (the stage's base in).
+struct LaneAddress {
+  uint32_t k;       // its 16 bytes (D = 64: 8) of K row g
+  uint32_t k_far;   // D = 256: those of the row's other half
+  uint32_t v0, v1;  // its bytes of V rows 2j and 2j + 1
+  uint32_t p;       // (scale, zero) of token g
+  __device__ __forceinline__ LaneAddress operator+(uint32_t x) const {
+    return LaneAddress{k + x, k_far + x, v0 + x, v1 + x, p + x};
+  }
+};
+
+template <int D>
+__device__ __forceinline__ LaneAddress lane_address(uint32_t base, int g, int j) {
+  LaneAddress a;
+  const uint32_t values = base + 2 * Shape<D>::kUnit;
+  const uint32_t swizzle = 32u * (D == 64 ? (j >> 1) & 1 : j);
+  const uint32_t v = uint32_t(D * j + (D / 16) * g) ^ swizzle;  // row 2j has D/2 bytes
+  a.v0 = values + v;
+  a.v1 = values + (v ^ (D / 2));
+  a.k = base + (D / 2) * g + (D == 256 ? 16 * (j ^ (4 * (g & 1))) : (D / 8) * j);
+  a.k_far = D == 256 ? base + 128 * g + (16 * (j ^ (4 * (g & 1))) ^ 64) : 0u;
+  a.p = base + 4 * Shape<D>::kUnit + 4 * g;
+  return a;
+}
+
+// K words of row g + 8 * kHigh of unit kUnitAt.
+template <int D, int kUnitAt, int kHigh>
+__device__ __forceinline__ void key_words(const LaneAddress& a, uint32_t (&w)[D / 32]) {
+  constexpr int at = kUnitAt * Shape<D>::kUnit + kHigh * 4 * D;
+  if constexpr (D == 64) {
+    const uint2 v = lds64<at>(a.k);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    const uint4 v = lds128<at>(a.k);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    if constexpr (D == 256) {
+      const uint4 u = lds128<at>(a.k_far);
+      w[4] = u.x, w[5] = u.y, w[6] = u.z, w[7] = u.w;
     }
+  }
+}
+
+// V words of rows 2j + kOdd + 8 * kHigh.
+template <int D, int kUnitAt, int kHigh>
+__device__ __forceinline__ void value_words(uint32_t a, uint32_t (&w)[D / 64]) {
+  constexpr int at = kUnitAt * Shape<D>::kUnit + kHigh * 4 * D;
+  if constexpr (D == 64) {
+    w[0] = lds32<at>(a);
+  } else if constexpr (D == 128) {
+    const uint2 v = lds64<at>(a);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    const uint4 v = lds128<at>(a);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+}
+
+// q . c of one unit's 16 tokens with the tile's rows.
+template <int D, int NT, int U>
+__device__ __forceinline__ void unit_scores(const LaneAddress& at, const TileShared<D, NT>& sh,
+                                            const uint2* qreg, float (&x)[NT][4]) {
+  constexpr int kW = D / 32;
+  uint32_t lo[kW], hi[kW];
+  key_words<D, U, 0>(at, lo);
+  key_words<D, U, 1>(at, hi);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[u][n][i] = 0.f;
+    for (int i = 0; i < 4; ++i) x[n][i] = 0.f;
 #pragma unroll
-    for (int w = 0; w < kKW; ++w) {
+  for (int w = 0; w < kW; ++w) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t r0 = h ? kw[0][w] >> 8 : kw[0][w], r1 = h ? kw[1][w] >> 8 : kw[1][w];
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t r0 = h ? lo[w] >> 8 : lo[w], r1 = h ? hi[w] >> 8 : hi[w];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint2 q = NT == 1 ? qreg[2 * w + h] : sh.q[n][2 * w + h][lane];
-          mma(x[u][n], r0 & kEven, r1 & kEven, r0 & kOdd, r1 & kOdd, q.x, q.y);
-        }
+      for (int n = 0; n < NT; ++n) {
+        const uint2 q = NT == 1 ? qreg[2 * w + h] : sh.q[n][2 * w + h][threadIdx.x % 32];
+        mma(x[n], r0 & kEven, r1 & kEven, r0 & kOdd, r1 & kOdd, q.x, q.y);
       }
     }
   }
-  // Scores in powers of two; this thread's tokens are g and g + 8 of each unit.
-  float top[NT][2];
-  float vs[AB][2], vz[AB][2], most = 0.f;
+}
+
+// Adds one unit's weights times its codes.
+template <int D, int NT, int U>
+__device__ __forceinline__ void unit_values(const LaneAddress& at, const uint32_t (&b)[NT][2],
+                                            WarpState<D, NT>& st) {
+  constexpr int kW = D / 64;
+  uint32_t w0[kW], w1[kW], w2[kW], w3[kW];
+  value_words<D, U, 0>(at.v0, w0);
+  value_words<D, U, 0>(at.v1, w1);
+  value_words<D, U, 1>(at.v0, w2);
+  value_words<D, U, 1>(at.v1, w3);
+#pragma unroll
+  for (int w = 0; w < kW; ++w)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // Byte e of tokens 2j and 2j + 1, each in the low end of a half.
+      const uint32_t select = 0x0400u + 0x0101u * e;
+      const uint32_t p = __byte_perm(w0[w], w1[w], select), q = __byte_perm(w2[w], w3[w], select);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        mma(st.o[n][4 * w + e], p & kEven, p & kOdd, q & kEven, q & kOdd, b[n][0], b[n][1]);
+    }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    mma(st.ps[n], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, b[n][0], b[n][1]);
+}
+
+// What a thread keeps of the tile's rows (its columns 2j, 2j + 1 of each eight).
+template <int NT>
+struct Columns {
+  float2 factor[NT];  // on the raw score: scale * log2(e) and the powers of two
+  float2 sum[NT];     // sum(q), in the raw score's unit
+  int pos[NT][2];
+};
+
+// kAb units from unit U of the stage on: scores, softmax, products.  `number` are the
+// units' numbers in the sequence, -1 for one that is not there.
+template <int D, int NT, int U, int kAb, bool kMasked>
+__device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared<D, NT>& sh,
+                                             const uint2* qreg, const LaneAddress& at,
+                                             const int (&number)[2], const Columns<NT>& col,
+                                             const Span& v, WarpState<D, NT>& st) {
+  const int lane = threadIdx.x % 32, g = lane / 4;
+  float x[kAb][NT][4];
+  unit_scores<D, NT, U>(at, sh, qreg, x[0]);
+  if constexpr (kAb == 2) unit_scores<D, NT, 1>(at, sh, qreg, x[1]);
+  // (scale, zero) of tokens g and g + 8 of each unit: K, then V.
+  uint32_t kp[kAb][2], vp[kAb][2];
+  kp[0][0] = lds32<64 * U>(at.p), kp[0][1] = lds32<64 * U + 32>(at.p);
+  vp[0][0] = lds32<128 + 64 * U>(at.p), vp[0][1] = lds32<128 + 64 * U + 32>(at.p);
+  if constexpr (kAb == 2) {
+    kp[1][0] = lds32<64>(at.p), kp[1][1] = lds32<96>(at.p);
+    vp[1][0] = lds32<192>(at.p), vp[1][1] = lds32<224>(at.p);
+  }
+  float top[NT][2], vs[kAb][2], vz[kAb][2], most = 0.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = kNegInf;
 #pragma unroll
-  for (int u = 0; u < AB; ++u)
+  for (int u = 0; u < kAb; ++u)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int at = (unit0 + u) * 64 + (g + 8 * r) * 4;
-      const float2 k = __half22float2(*reinterpret_cast<const __half2*>(params + at));
-      const float2 w = __half22float2(*reinterpret_cast<const __half2*>(params + 128 + at));
+      const float2 k = half2_at(kp[u][r]), w = half2_at(vp[u][r]);
       vs[u][r] = w.x;
       vz[u][r] = fmaf(7.5f, w.x, w.y);
-      const int t = number[u] * 16 + g + 8 * r;
+      const int unit = number[U + u], t = unit * 16 + g + 8 * r;
       // Only of tokens that some row sees: what lies behind a sequence may be anything.
-      if (!kMasked || (number[u] >= 0 && t <= v.p_hi && (t > v.p_lo - a.window || t < a.sinks)))
+      if (!kMasked || (unit >= 0 && t <= v.p_hi && (t > v.p_lo - a.window || t < a.sinks)))
         most = fmaxf(most, fabsf(w.x));
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float& y = x[u][n][2 * r + c];
-          y = fmaf(k.x, y * factor[n][c], k.y * qsum[n][c]);
+          y = fmaf(k.x, y, k.y * (c ? col.sum[n].y : col.sum[n].x));
           if constexpr (kMasked) {
-            const int p = pos[n][c];
-            const bool seen = number[u] >= 0 && t <= p && (t > p - a.window || t < a.sinks);
+            const int p = col.pos[n][c];
+            const bool seen = unit >= 0 && t <= p && (t > p - a.window || t < a.sinks);
             y = seen ? y : kNegInf;
           }
           top[n][c] = fmaxf(top[n][c], y);
         }
     }
   // Move the reference point where a score passes it by 2^8, or the weights
-  // would leave fp16.
+  // would leave fp16.  The factors are positive, so raw scores have the order.
   bool move = !(most * st.c <= 64.f) || st.c == 0.f;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) move |= top[n][0] > st.m[n][0] + 8.f || top[n][1] > st.m[n][1] + 8.f;
+  for (int n = 0; n < NT; ++n) {
+    top[n][0] *= col.factor[n].x;
+    top[n][1] *= col.factor[n].y;
+    move |= top[n][0] > st.m[n].x + 8.f || top[n][1] > st.m[n].y + 8.f;
+  }
   if (__any_sync(~0u, move)) {
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
@@ -395,14 +516,15 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
       float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float t = fmaxf(top[n][c], st.m[n][c]);
+        float& m = c ? st.m[n].y : st.m[n].x;
+        float t = fmaxf(top[n][c], m);
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
-        f[c] = t == kNegInf ? 1.f : ex2(st.m[n][c] - t);
-        st.m[n][c] = t;
-        st.l[n][c] *= f[c];
-        st.z[n][c] *= f[c];
+        f[c] = t == kNegInf ? 1.f : ex2(m - t);
+        m = t;
       }
+      st.l[n].x *= f[0], st.l[n].y *= f[1];
+      st.z[n][0] *= f[0], st.z[n][1] *= f[1];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         st.ps[n][i] *= f[i % 2] * ratio;
@@ -411,68 +533,38 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
       }
     }
   }
-  uint32_t b[AB][NT][2];
+  uint32_t b[kAb][NT][2];
 #pragma unroll
-  for (int u = 0; u < AB; ++u)
+  for (int u = 0; u < kAb; ++u)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float weight = vs[u][r] * st.c;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float y[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float m = kMasked && st.m[n][c] == kNegInf ? 0.f : st.m[n][c];
-          const float p = ex2(x[u][n][2 * r + c] - m);
-          st.l[n][c] += p;
-          if (kMasked && p == 0.f) {  // a hidden token's scale and zero may be anything
-            y[c] = 0.f;
-          } else {
-            y[c] = p * weight;
-            st.z[n][c] = fmaf(p, vz[u][r], st.z[n][c]);
-          }
+        float2 m = st.m[n];
+        if (kMasked) {
+          m.x = m.x == kNegInf ? 0.f : m.x;
+          m.y = m.y == kNegInf ? 0.f : m.y;
         }
+        float2 p = fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]), col.factor[n],
+                        make_float2(-m.x, -m.y));
+        p.x = ex2(p.x), p.y = ex2(p.y);
+        st.l[n] = add2(st.l[n], p);
+        float y[2] = {p.x * weight, p.y * weight};
+        float z[2] = {fmaf(p.x, vz[u][r], st.z[n][0]), fmaf(p.y, vz[u][r], st.z[n][1])};
+        if (kMasked) {  // a hidden token's scale and zero may be anything
+          if (p.x == 0.f) y[0] = 0.f, z[0] = st.z[n][0];
+          if (p.y == 0.f) y[1] = 0.f, z[1] = st.z[n][1];
+        }
+        st.z[n][0] = z[0], st.z[n][1] = z[1];
         const __half2 h = __floats2half2_rn(y[0], y[1]);
-        __builtin_memcpy(&b[u][n][r], &h, 4);
-        b[u][n][r] = transpose8x8(b[u][n][r]);
+        uint32_t bits;
+        __builtin_memcpy(&bits, &h, 4);
+        b[u][n][r] = transpose8x8(bits);
       }
     }
-#pragma unroll
-  for (int u = 0; u < AB; ++u) {
-    const uint8_t* unit = values + (unit0 + u) * kUnit;
-    uint32_t vw[4][kVW];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = 2 * j + (r & 1) + 8 * (r >> 1);
-      if constexpr (D == 64) {
-        vw[r][0] = *reinterpret_cast<const uint32_t*>(
-            unit + ((t * 32 + 4 * g) ^ (32 * ((t >> 2) & 1))));
-      } else if constexpr (D == 128) {
-        const uint2 v = *reinterpret_cast<const uint2*>(
-            unit + ((t * 64 + 8 * g) ^ (32 * ((t >> 1) & 3))));
-        vw[r][0] = v.x, vw[r][1] = v.y;
-      } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(
-            unit + ((t * 128 + 16 * g) ^ (32 * ((t >> 1) & 3))));
-        vw[r][0] = v.x, vw[r][1] = v.y, vw[r][2] = v.z, vw[r][3] = v.w;
-      }
-    }
-#pragma unroll
-    for (int w = 0; w < kVW; ++w)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // Tokens 2j, 2j+1 side by side: the low or high halves of their words.
-        const uint32_t sel = e < 2 ? 0x5410u : 0x7632u;
-        uint32_t p = __byte_perm(vw[0][w], vw[1][w], sel), q = __byte_perm(vw[2][w], vw[3][w], sel);
-        if (e % 2) p >>= 8, q >>= 8;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          mma(st.o[n][4 * w + e], p & kEven, p & kOdd, q & kEven, q & kOdd, b[u][n][0], b[u][n][1]);
-      }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      mma(st.ps[n], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, b[u][n][0], b[u][n][1]);
-  }
+  unit_values<D, NT, U>(at, b[0], st);
+  if constexpr (kAb == 2) unit_values<D, NT, 1>(at, b[1], st);
 }
 
 // Four dimensions of one row's result: sum / l and log-sum-exp; zeros and -inf
@@ -504,7 +596,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const Seq& s, int r
 // warps' results are joined.  `slot` < 0: the result is the tile's output,
 // otherwise it goes to that place of the workspace.
 template <typename T, int D, int NT>
-__device__ void attend_segment(const AttnArgs& a, TileShared<D, NT>& sh, uint8_t* ring, int b,
+__device__ __forceinline__ void attend_segment(const AttnArgs& a, TileShared<D, NT>& sh, uint8_t* ring, int b,
                                const Seq& s, const Span& v, int row0, int rows, int head, int u0,
                                int u1, int slot) {
   using S = Shape<D>;
@@ -515,90 +607,86 @@ __device__ void attend_segment(const AttnArgs& a, TileShared<D, NT>& sh, uint8_t
   const int steps = pairs > warp ? (pairs - warp + kWarps - 1) / kWarps : 0;
   const int32_t* table = a.tables + int64_t(b) * a.table_stride;
 
-  // Block ids of the next 16 steps, two units each, one in every lane.
-  auto fetch_ids = [&](int step, int& id, int& within) {
+  // Where the units of the next 16 steps are, two a step, one in every lane:
+  // byte offset in the pages and token in the page.  `have` has a bit for each.
+  struct Units {
+    int64_t offset;
+    int within;
+    uint32_t have;
+  };
+  auto fetch = [&](int step) {
+    Units f{0, 0, 0u};
     const int i = u0 + 2 * (warp + kWarps * (step + lane / 2)) + lane % 2;
-    id = -1;
-    within = 0;
-    if (i < u1) {
+    bool real = i < u1;
+    if (real) {
       const int n = i < v.sink_units ? i : i + v.gap;
       const int page = a.upp_shift >= 0 ? n >> a.upp_shift : n / a.upp;
-      within = n - page * a.upp;
-      id = table[page];
-      if (id < 0 || id >= a.cache.num_blocks) {
-        id = -1;
-        atomicExch(&g_q4_status, 5 /* KVX_ERR_BLOCK_ID */);
-      }
+      const int id = table[page];
+      f.within = n - page * a.upp;
+      real = id >= 0 && id < a.cache.num_blocks;
+      if (real) f.offset = id * a.cache.stride + f.within * S::kUnit;
+      else atomicExch(&g_q4_status, 5 /* KVX_ERR_BLOCK_ID */);
     }
+    f.have = __ballot_sync(~0u, real);
+    return f;
   };
-  int id, within, next_id = -1, next_within = 0;
-  fetch_ids(0, id, within);
-  if (steps > 16) fetch_ids(16, next_id, next_within);
+  Units now = fetch(0), later{0, 0, 0u};
+  if (steps > 16) later = fetch(16);
   uint32_t there = 0;  // which units of the steps in flight are there, two bits a step
 
-  auto load_step = [&](int step, int buffer) {
+  // This lane's part of the copies: 16-byte pieces lane, lane + 32, ... of each
+  // unit's codes, and one piece of the four runs of scales and zeros.
+  const int64_t head_at = int64_t(head) * a.cache.head_bytes;
+  const uint8_t* key_from = a.cache.pages[0] + head_at + 16 * lane;
+  const uint8_t* value_from = a.cache.pages[1] + head_at + 16 * lane;
+  const int param_unit = (lane / 4) % 2;
+  const uint8_t* param_from = a.cache.pages[(lane / 8) % 2] + head_at +
+                              a.cache.block_size * (D / 2) + 16 * (lane % 4);
+  auto load_step = [&](int step, uint32_t dst) {
     const int at = 2 * (step % 16);
-    const uint32_t dst = mine_s + buffer * S::kStage;
-    const int ids[2] = {__shfl_sync(~0u, id, at), __shfl_sync(~0u, id, at + 1)};
-    const int in[2] = {__shfl_sync(~0u, within, at), __shfl_sync(~0u, within, at + 1)};
+    const uint32_t bits = (now.have >> at) & 3u;
+    there = (there << 2) | bits;
+    const int64_t offset[2] = {__shfl_sync(~0u, now.offset, at),
+                               __shfl_sync(~0u, now.offset, at + 1)};
+    const int within = __shfl_sync(~0u, now.within, at + param_unit);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint8_t* pages = a.cache.pages[t] + int64_t(head) * a.cache.head_bytes;
+    for (int u = 0; u < 2; ++u) {
+      const int size = (bits >> u) & 1u ? 16 : 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const bool real = ids[u] >= 0;
-        const uint8_t* src =
-            pages + int64_t(real ? ids[u] : 0) * a.cache.stride[t] + in[u] * S::kUnit;
-#pragma unroll
-        for (int i = 0; i < S::kUnit / 512; ++i) {
-          const int c = lane + 32 * i;
-          int swizzle = 0;  // so that the fragments' reads meet no bank twice
-          if (t == 1)
-            swizzle = D == 64 ? 2 * ((c >> 3) & 1) : D == 128 ? 2 * ((c >> 3) & 3) : 2 * ((c >> 4) & 3);
-          else if (D == 256)
-            swizzle = 4 * ((c >> 3) & 1);
-          copy16(dst + (2 * t + u) * S::kUnit + 16 * (c ^ swizzle), src + 16 * c, real);
-        }
+      for (int i = 0; i < S::kUnit / 512; ++i) {
+        // The pieces' places are permuted so that the fragments' reads meet no bank twice.
+        const int c = lane + 32 * i;
+        const int kc = D == 256 ? c ^ (4 * ((c >> 3) & 1)) : c;
+        const int vc = c ^ (D == 64    ? 2 * ((c >> 3) & 1)
+                            : D == 128 ? 2 * ((c >> 3) & 3)
+                                       : 2 * ((c >> 4) & 3));
+        copy16(dst + u * S::kUnit + 16 * kc, key_from + offset[u] + 512 * i, size);
+        copy16(dst + (2 + u) * S::kUnit + 16 * vc, value_from + offset[u] + 512 * i, size);
       }
     }
-    if (lane < 16) {  // scales and zeros: 64 bytes for each unit and tensor
-      const int t = lane / 8, u = (lane / 4) % 2;
-      const bool real = ids[u] >= 0;
-      const uint8_t* src = a.cache.pages[t] + int64_t(real ? ids[u] : 0) * a.cache.stride[t] +
-                           int64_t(head) * a.cache.head_bytes + a.cache.block_size * (D / 2) +
-                           in[u] * 64 + 16 * (lane % 4);
-      copy16(dst + 4 * S::kUnit + 16 * lane, src, real);
-    }
-    there = (there << 2) | (ids[0] >= 0 ? 1u : 0u) | (ids[1] >= 0 ? 2u : 0u);
-  };
-  auto advance_ids = [&](int step) {  // before the first load of a new group of 16
-    if (step % 16 == 0 && step > 0) {
-      id = next_id;
-      within = next_within;
-      next_id = -1;
-      if (step + 16 < steps) fetch_ids(step + 16, next_id, next_within);
-    }
+    if (lane < 16)
+      copy16(dst + 4 * S::kUnit + 16 * lane,
+             param_from + offset[param_unit] - within * (S::kUnit - 64),
+             (bits >> param_unit) & 1u ? 16 : 0);
   };
 
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
-    if (i < steps) load_step(i, i);
+    if (i < steps) load_step(i, mine_s + i * S::kStage);
     else there <<= 2;
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   load_queries<T, D, NT>(a, s, row0, rows, head, sh);
   __syncthreads();
 
-  float factor[NT][2], qsum[NT][2];
-  int pos[NT][2];
+  Columns<NT> col;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      factor[n][c] = sh.factor[8 * n + 2 * j + c];
-      qsum[n][c] = sh.sum[8 * n + 2 * j + c];
-      pos[n][c] = sh.pos[8 * n + 2 * j + c];
-    }
+  for (int n = 0; n < NT; ++n) {
+    const int c = 8 * n + 2 * j;
+    col.factor[n] = make_float2(sh.factor[c], sh.factor[c + 1]);
+    col.sum[n] = make_float2(sh.sum[c], sh.sum[c + 1]);
+    col.pos[n][0] = sh.pos[c], col.pos[n][1] = sh.pos[c + 1];
+  }
   uint2 qreg[NT == 1 ? D / 16 : 1];
   if constexpr (NT == 1) {
 #pragma unroll
@@ -608,8 +696,8 @@ __device__ void attend_segment(const AttnArgs& a, TileShared<D, NT>& sh, uint8_t
   st.c = 0.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) st.m[n][c] = kNegInf, st.l[n][c] = 0.f, st.z[n][c] = 0.f;
+    st.m[n] = make_float2(kNegInf, kNegInf), st.l[n] = make_float2(0.f, 0.f);
+    st.z[n][0] = st.z[n][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       st.ps[n][i] = 0.f;
@@ -618,48 +706,47 @@ __device__ void attend_segment(const AttnArgs& a, TileShared<D, NT>& sh, uint8_t
     }
   }
 
-  int buffer = 0;
-  for (int step = 0; step < steps; ++step) {
+  // Pairs [plain_from, plain_from + plain_units) need no mask: behind no row,
+  // and inside every row's window.
+  const int plain_from = max(v.sink_units, (max(v.p_hi - a.window + 1, 0) + 15) / 16 - v.gap);
+  const unsigned plain_units = unsigned(max((v.p_lo + 1) / 16 - v.gap - plain_from - 1, 0));
+  const LaneAddress lane_at = lane_address<D>(mine_s, g, j);
+  uint32_t buffer = 0, ahead = (kStages - 1) * S::kStage;  // bytes into the ring
+  int i = u0 + 2 * warp;
+  for (int step = 0; step < steps; ++step, i += 2 * kWarps) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncwarp();
-    {
-      const int next = step + kStages - 1;
-      int to = buffer + kStages - 1;
-      if (to >= kStages) to -= kStages;
-      advance_ids(next);
-      if (next < steps) load_step(next, to);
-      else there <<= 2;
-      asm volatile("cp.async.commit_group;" ::: "memory");
+    const int next = step + kStages - 1;
+    if (next % 16 == 0) {
+      now = later;
+      if (next + 16 < steps) later = fetch(next + 16);
     }
+    if (next < steps) load_step(next, mine_s + ahead);
+    else there <<= 2;
+    asm volatile("cp.async.commit_group;" ::: "memory");
     const uint32_t bits = (there >> (2 * (kStages - 1))) & 3u;
-    const int i = u0 + 2 * (warp + kWarps * step);
-    int number[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      number[u] = (bits >> u) & 1u ? (i + u < v.sink_units ? i + u : i + u + v.gap) : -1;
-    const int last = number[1] * 16 + 15, first = number[0] * 16;
-    // Whole pairs need no mask: behind no row, and inside every row's window
-    // or among the sinks.
-    const bool plain = bits == 3u && last <= v.p_lo &&
-                       (first > v.p_hi - a.window || last < a.sinks);
-    const uint8_t* stage = mine + buffer * S::kStage;
+    const bool plain = bits == 3u && unsigned(i - plain_from) < plain_units;
+    const LaneAddress at = lane_at + buffer;
+    int number[2] = {0, 0};
+    if (!plain) {
+      number[0] = bits & 1u ? (i < v.sink_units ? i : i + v.gap) : -1;
+      number[1] = bits & 2u ? (i + 1 < v.sink_units ? i + 1 : i + 1 + v.gap) : -1;
+    }
     if constexpr (NT <= 2) {
       if (plain)
-        attend_units<D, NT, 2, false>(a, sh, qreg, stage, 0, number, factor, qsum, pos, v, st);
+        attend_units<D, NT, 0, 2, false>(a, sh, qreg, at, number, col, v, st);
       else
-        attend_units<D, NT, 2, true>(a, sh, qreg, stage, 0, number, factor, qsum, pos, v, st);
+        attend_units<D, NT, 0, 2, true>(a, sh, qreg, at, number, col, v, st);
+    } else if (plain) {
+      attend_units<D, NT, 0, 1, false>(a, sh, qreg, at, number, col, v, st);
+      attend_units<D, NT, 1, 1, false>(a, sh, qreg, at, number, col, v, st);
     } else {
-#pragma unroll 1
-      for (int u = 0; u < 2; ++u) {
-        const int one[1] = {u ? number[1] : number[0]};
-        if (plain)
-          attend_units<D, NT, 1, false>(a, sh, qreg, stage, u, one, factor, qsum, pos, v, st);
-        else
-          attend_units<D, NT, 1, true>(a, sh, qreg, stage, u, one, factor, qsum, pos, v, st);
-      }
+      attend_units<D, NT, 0, 1, true>(a, sh, qreg, at, number, col, v, st);
+      attend_units<D, NT, 1, 1, true>(a, sh, qreg, at, number, col, v, st);
     }
     __syncwarp();
-    if (++buffer == kStages) buffer = 0;
+    buffer = buffer + S::kStage == S::kWarpBytes ? 0u : buffer + S::kStage;
+    ahead = ahead + S::kStage == S::kWarpBytes ? 0u : ahead + S::kStage;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 
@@ -668,14 +755,15 @@ __device__ void attend_segment(const AttnArgs& a, TileShared<D, NT>& sh, uint8_t
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
+      float l = c ? st.l[n].y : st.l[n].x;
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) {
-        st.l[n][c] += __shfl_xor_sync(~0u, st.l[n][c], d);
+        l += __shfl_xor_sync(~0u, l, d);
         st.z[n][c] += __shfl_xor_sync(~0u, st.z[n][c], d);
       }
       if (g == 0) {
-        sh.m[warp][8 * n + 2 * j + c] = st.m[n][c];
-        sh.l[warp][8 * n + 2 * j + c] = st.l[n][c];
+        sh.m[warp][8 * n + 2 * j + c] = c ? st.m[n].y : st.m[n].x;
+        sh.l[warp][8 * n + 2 * j + c] = l;
       }
     }
   const float back = st.c > 0.f ? 1.f / st.c : 0.f;
@@ -731,9 +819,18 @@ __device__ void attend_segment(const AttnArgs& a, TileShared<D, NT>& sh, uint8_t
   __syncthreads();  // before the ring and the rows are used again
 }
 
-// What a sequence adds to the work: tiles of query rows x kv heads, each taken
-// as long as the longest of the sequence's tiles (at least one unit, so that
-// rows that see nothing are written too).
+// Rows of a tile that see nothing.
+template <typename T, int D>
+__device__ __forceinline__ void store_nothing(const AttnArgs& a, const Seq& s, int row0, int rows,
+                                              int head) {
+  for (int e = threadIdx.x; e < rows * (D / 4); e += kThreads)
+    store_row<T>(a, s, row0 + e / (D / 4), head, e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f),
+                 kNegInf, 0.f);
+}
+
+// What a sequence adds to the work: items of one tile of query rows with one kv
+// head, each counted as long as the longest of the sequence's tiles, behind
+// kItemUnits for what an item costs besides.
 struct Work {
   Seq s;
   int rows, tiles, units;
@@ -746,15 +843,31 @@ __device__ __forceinline__ Work work_of(const AttnArgs& a, int b) {
   w.s = seq_of(a, b);
   w.rows = w.s.count * a.group;
   w.tiles = (w.rows + ROWS - 1) / ROWS;
-  w.units = max(span_of(a, w.s, 0, w.rows).units, 1);
-  w.total = int64_t(w.units) * w.tiles * a.cache.kv_heads;
+  w.units = span_of(a, w.s, 0, w.rows).units;
+  w.total = int64_t(w.units + kItemUnits) * w.tiles * a.cache.kv_heads;
   return w;
 }
 
-// All units of the call, [tile x head][unit] of one sequence after the other,
+__device__ __forceinline__ int64_t share_of(int64_t total, int shares) {
+  return max(int64_t(kMinUnits + kItemUnits), (total + shares - 1) / shares);
+}
+
+// Item and offset in it of a position of a sequence's work.
+__device__ __forceinline__ void item_of(const Work& w, int64_t in, int* item, int* off) {
+  const int length = w.units + kItemUnits;
+  if (in < (int64_t(1) << 31)) {  // the common case: no 64-bit division
+    *item = int(unsigned(in) / unsigned(length));
+    *off = int(unsigned(in) - unsigned(*item) * unsigned(length));
+  } else {
+    *item = int(in / length);
+    *off = int(in - int64_t(*item) * length);
+  }
+}
+
+// All work of the call, [kv head][tile][units] of one sequence after the other,
 // in equal shares: one for each CTA of a grid that is resident at once.  A
-// share that begins or ends inside an item leaves a partial result in the
-// workspace (at most two for a CTA), which q4_join brings together.
+// share that begins or ends among an item's units leaves a partial result in
+// the workspace (at most two for a CTA), which q4_join brings together.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, NT <= 2 && D <= 128 ? 2 : 1)
     q4_attend(const __grid_constant__ AttnArgs a) {
@@ -762,12 +875,17 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 && D <= 128 ? 2 : 1)
   __shared__ TileShared<D, NT> sh;
   constexpr int kRows = 8 * NT;
   asm volatile("griddepcontrol.launch_dependents;");
-  auto cost = [&](int b) { return work_of<kRows>(a, b).total; };
-  const int64_t total = block_total(cost, a.batch, sh.scan);
-  const int64_t share = max(int64_t(kMinUnits), (total + gridDim.x - 1) / gridDim.x);
+  Place place;
+  int64_t share = 0;
+  const int64_t total = block_locate(
+      [&](int b) { return work_of<kRows>(a, b).total; }, a.batch,
+      [&](int64_t all) {
+        share = share_of(all, gridDim.x);
+        return share * blockIdx.x;
+      },
+      sh.scan, &sh.place, &place);
   const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
   if (begin >= end) return;
-  const Place place = block_locate(cost, a.batch, begin, sh.scan, &sh.place);
   int b = place.index;
   int64_t before = place.before, pos = begin;
   while (pos < end && b < a.batch) {
@@ -776,15 +894,22 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 && D <= 128 ? 2 : 1)
       ++b;
       continue;
     }
-    const int item = int((pos - before) / w.units), off = int((pos - before) % w.units);
-    const int n = int(min(int64_t(w.units - off), end - pos));
+    int item, off;
+    item_of(w, pos - before, &item, &off);
+    const int n = int(min(int64_t(w.units + kItemUnits - off), end - pos));
     const int head = item / w.tiles, row0 = (item % w.tiles) * kRows;
     const int rows = min(kRows, w.rows - row0);
-    const Span v = span_of(a, w.s, row0, rows);
-    const bool whole = off == 0 && n == w.units;
-    attend_segment<T, D, NT>(a, sh, ring, b, w.s, v, row0, rows, head, min(off, v.units),
-                             min(off + n, v.units),
-                             whole ? -1 : 2 * int(blockIdx.x) + (pos == begin ? 0 : 1));
+    // Units of this share; the item's first kItemUnits positions stand for none.
+    const int u0 = max(off - kItemUnits, 0), u1 = max(off + n - kItemUnits, 0);
+    if (w.units == 0) {
+      if (off == 0) store_nothing<T, D>(a, w.s, row0, rows, head);
+    } else if (u1 > u0) {
+      const Span v = span_of(a, w.s, row0, rows);
+      const bool whole = u0 == 0 && u1 == w.units;
+      attend_segment<T, D, NT>(a, sh, ring, b, w.s, v, row0, rows, head, min(u0, v.units),
+                               min(u1, v.units),
+                               whole ? -1 : 2 * int(blockIdx.x) + (pos == begin ? 0 : 1));
+    }
     pos += n;
     if (pos - before == w.total) {
       before = pos;
@@ -793,60 +918,155 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 && D <= 128 ? 2 : 1)
   }
 }
 
-// Joins the partial results of items that several CTAs shared.  Block k looks
-// at the border behind share k and works when it is the first one inside an
-// item; the pieces are summed in their order, so results do not vary.
-template <typename T, int D, int NT>
+// The pieces of an item that starts at `start`: shares first .. last hold units
+// of it.  A share's piece is its first (even slot) where the share begins inside
+// the item or at its start.
+struct Pieces {
+  int64_t start, share, first, last;
+  __device__ __forceinline__ int64_t slot(int64_t k) const {
+    return 2 * k + (start > k * share ? 1 : 0);
+  }
+};
+
+__device__ __forceinline__ Pieces pieces_of(const Work& w, int64_t start, int64_t share) {
+  return Pieces{start, share, (start + kItemUnits) / share,
+                (start + kItemUnits + w.units - 1) / share};
+}
+
+// Joins one row's pieces, those of warp `part` of `parts`, in their order.
+template <int D>
+__device__ __forceinline__ void join_row(const AttnArgs& a, const Pieces& p, int kRows, int r,
+                                         int part, int parts, float& m, float& l,
+                                         float4 (&o)[(D + 127) / 128]) {
+  const int lane = threadIdx.x % 32;
+  m = kNegInf;
+  for (int64_t k = p.first + lane; k <= p.last; k += 32)
+    m = fmaxf(m, a.part_ml[p.slot(k) * kRows + r].x);
+#pragma unroll
+  for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < (D + 127) / 128; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int64_t k = p.first + part; k <= p.last; k += parts) {
+    const int64_t at = p.slot(k) * kRows + r;
+    const float2 ml = a.part_ml[at];
+    float4 x[(D + 127) / 128];
+#pragma unroll
+    for (int i = 0; i < (D + 127) / 128; ++i) {
+      const int d = 128 * i + 4 * lane;
+      x[i] = d < D ? *reinterpret_cast<const float4*>(a.part_o + at * D + d)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    // A piece without a finite score counts for nothing, unless a NaN is in it.
+    const float f = ml.x == kNegInf ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - m);
+    if (f != 0.f) {
+      l = fmaf(f, ml.y, l);
+#pragma unroll
+      for (int i = 0; i < (D + 127) / 128; ++i) {
+        o[i].x = fmaf(f, x[i].x, o[i].x), o[i].y = fmaf(f, x[i].y, o[i].y);
+        o[i].z = fmaf(f, x[i].z, o[i].z), o[i].w = fmaf(f, x[i].w, o[i].w);
+      }
+    }
+  }
+}
+
+// Joins the partial results of items that several CTAs shared; the pieces are
+// summed in an order that does not vary.  Two forms:
+//   kByRow false: block k looks at the border behind share k and works when it
+//     is the first border among an item's units; a warp takes a row.
+//   kByRow true: a block for each row of each item, its warps share the pieces:
+//     for few items with many pieces, where a warp alone would take long.
+template <typename T, int D, int NT, bool kByRow>
 __global__ void __launch_bounds__(kThreads) q4_join(const __grid_constant__ AttnArgs a,
                                                     int shares) {
   __shared__ int64_t scan[kWarps];
   __shared__ Place found;
+  __shared__ float4 part[kByRow ? kWarps : 1][(D + 127) / 128][32];
+  __shared__ float part_l[kWarps];
   constexpr int kRows = 8 * NT;
-  auto cost = [&](int b) { return work_of<kRows>(a, b).total; };
-  const int64_t total = block_total(cost, a.batch, scan);
-  const int64_t share = max(int64_t(kMinUnits), (total + shares - 1) / shares);
-  const int64_t border = share * (int64_t(blockIdx.x) + 1);
-  const Place place = block_locate(cost, a.batch, border, scan, &found);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (border >= total || place.index >= a.batch) return;
-  const Work w = work_of<kRows>(a, place.index);
-  const int item = int((border - place.before) / w.units);
-  const int64_t start = place.before + int64_t(item) * w.units;
-  const int64_t k0 = start / share, k1 = (start + w.units - 1) / share;
-  if (start == border || k0 != blockIdx.x) return;
-  const int row0 = (item % w.tiles) * kRows, rows = min(kRows, w.rows - row0);
-  const int lane = threadIdx.x % 32;
-  auto slot_of = [&](int64_t k) { return 2 * k + (k == k0 && start != k0 * share ? 1 : 0); };
-  for (int r = threadIdx.x / 32; r < rows; r += kWarps) {
-    float m = kNegInf;
-    for (int64_t k = k0 + lane; k <= k1; k += 32) m = fmaxf(m, a.part_ml[slot_of(k) * kRows + r].x);
-#pragma unroll
-    for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-    float l = 0.f;
-    float4 o[(D + 127) / 128] = {};
-    for (int64_t k = k0; k <= k1; ++k) {
-      const int64_t at = slot_of(k) * kRows + r;
-      const float2 p = a.part_ml[at];
-      const float f = p.x == kNegInf ? (p.y == p.y ? 0.f : p.y) : ex2(p.x - m);
-      if (f != 0.f) {
-        l = fmaf(f, p.y, l);
-#pragma unroll
-        for (int i = 0; i < (D + 127) / 128; ++i) {
-          const int d = 128 * i + 4 * lane;
-          if (d < D) {
-            const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * D + d);
-            o[i].x = fmaf(f, x.x, o[i].x), o[i].y = fmaf(f, x.y, o[i].y);
-            o[i].z = fmaf(f, x.z, o[i].z), o[i].w = fmaf(f, x.w, o[i].w);
-          }
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  Place place;           // the item's sequence and the work before it
+  int64_t share = 0, start = 0;  // work before the item
+  bool none = false;
+  if constexpr (kByRow) {
+    // Few sequences: one thread walks them.
+    __shared__ int64_t walked[2];
+    if (threadIdx.x == 0) {
+      int64_t left = blockIdx.x / kRows, total = 0;
+      found = Place{a.batch, 0};
+      for (int b = 0; b < a.batch; ++b) {
+        const Work w = work_of<kRows>(a, b);
+        const int64_t items = int64_t(w.tiles) * a.cache.kv_heads;
+        if (left >= 0 && left < items) {
+          found = Place{b, total};
+          walked[1] = total + left * (w.units + kItemUnits);
         }
+        left -= items;
+        total += w.total;
       }
+      walked[0] = total;
     }
+    __syncthreads();
+    place = found;
+    share = share_of(walked[0], shares);
+    start = walked[1];
+    none = place.index >= a.batch;
+  } else {
+    const int64_t total = block_locate(
+        [&](int b) { return work_of<kRows>(a, b).total; }, a.batch,
+        [&](int64_t all) {
+          share = share_of(all, shares);
+          return share * (int64_t(blockIdx.x) + 1);
+        },
+        scan, &found, &place);
+    start = share * (int64_t(blockIdx.x) + 1);  // the border, for now
+    none = start >= total;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (none) return;
+  const Work w = work_of<kRows>(a, place.index);
+  if (w.units == 0) return;
+  int item, off;
+  item_of(w, start - place.before, &item, &off);
+  start -= off;
+  const Pieces p = pieces_of(w, start, share);
+  if (p.first == p.last || (!kByRow && p.first != blockIdx.x)) return;
+  const int row0 = (item % w.tiles) * kRows, rows = min(kRows, w.rows - row0);
+  const int head = item / w.tiles;
+  float m, l;
+  float4 o[(D + 127) / 128];
+  if (!kByRow) {
+    for (int r = warp; r < rows; r += kWarps) {
+      join_row<D>(a, p, kRows, r, 0, 1, m, l, o);
+#pragma unroll
+      for (int i = 0; i < (D + 127) / 128; ++i)
+        if (128 * i + 4 * lane < D)
+          store_row<T>(a, w.s, row0 + r, head, 128 * i + 4 * lane, o[i], m, l);
+    }
+    return;
+  }
+  const int r = blockIdx.x % kRows;
+  if (r >= rows) return;
+  join_row<D>(a, p, kRows, r, warp, kWarps, m, l, o);
+#pragma unroll
+  for (int i = 0; i < (D + 127) / 128; ++i) part[kByRow ? warp : 0][i][lane] = o[i];
+  if (lane == 0) part_l[warp] = l;
+  __syncthreads();
+  if (warp > 0) return;
+#pragma unroll
+  for (int k = 1; k < kWarps; ++k) {
+    l += part_l[k];
 #pragma unroll
     for (int i = 0; i < (D + 127) / 128; ++i) {
-      const int d = 128 * i + 4 * lane;
-      if (d < D) store_row<T>(a, w.s, row0 + r, item / w.tiles, d, o[i], m, l);
+      const float4 x = part[kByRow ? k : 0][i][lane];
+      o[i].x += x.x, o[i].y += x.y, o[i].z += x.z, o[i].w += x.w;
     }
   }
+#pragma unroll
+  for (int i = 0; i < (D + 127) / 128; ++i)
+    if (128 * i + 4 * lane < D)
+      store_row<T>(a, w.s, row0 + r, head, 128 * i + 4 * lane, o[i], m, l);
 }
 
 }  // namespace q4

@@ -28,7 +28,7 @@ static __device__ int g_q4_status;
 // Geometry of one cache (a K and a V tensor of one shape).
 struct Cache {
   uint8_t* pages[2];   // K, V
-  int64_t stride[2];   // bytes from one page to the next
+  int64_t stride;      // bytes from one page to the next, the same for both
   int64_t num_blocks;
   int kv_heads;
   int block_size;      // tokens of a page, a multiple of 16
@@ -118,10 +118,9 @@ __device__ __forceinline__ void store16(T* p, const T (&x)[16]) {
   }
 }
 
-// Where a slot's row of one head is in a tensor's pages.
-__device__ __forceinline__ int64_t row_offset(const Cache& c, int64_t stride, int64_t block,
-                                              int head) {
-  return block * stride + int64_t(head) * c.head_bytes;
+// One head's part of a page.
+__device__ __forceinline__ int64_t head_offset(const Cache& c, int64_t block, int head) {
+  return block * c.stride + int64_t(head) * c.head_bytes;
 }
 
 // Code of x in [0, 15]: rint((x - zero) / scale), ties to even, in real
@@ -212,8 +211,7 @@ __global__ void __launch_bounds__(kRowThreads) q4_write(const RowArgs a) {
         w[i / 8] |= code_of(to_float(x[s][i]), zero, scale, inv) << (4 * (i % 8));
     }
     if (live) {
-      uint8_t* page =
-          a.cache.pages[s] + row_offset(a.cache, a.cache.stride[s], block, head);
+      uint8_t* page = a.cache.pages[s] + head_offset(a.cache, block, head);
       *reinterpret_cast<uint2*>(page + within * (D / 2) + lane * 8) = make_uint2(w[0], w[1]);
       if (lane == 0)
         *reinterpret_cast<__half2*>(page + a.cache.block_size * (D / 2) + within * 4) =
@@ -246,8 +244,7 @@ __global__ void __launch_bounds__(kRowThreads) q4_read(const RowArgs a) {
   if (live) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const uint8_t* page =
-          a.cache.pages[s] + row_offset(a.cache, a.cache.stride[s], block, head);
+      const uint8_t* page = a.cache.pages[s] + head_offset(a.cache, block, head);
       w[s] = *reinterpret_cast<const uint2*>(page + within * (D / 2) + lane * 8);
       p[s] = *reinterpret_cast<const __half2*>(page + a.cache.block_size * (D / 2) + within * 4);
     }

@@ -83,9 +83,10 @@ def _cache(key_pages: torch.Tensor, value_pages: torch.Tensor, head_dim: int):
     ks, vs = key_pages.stride(), value_pages.stride()
     if (ks[2] != 1 or vs[2] != 1 or (heads > 1 and (ks[1] != size or vs[1] != size))):
         raise ValueError("the bytes of a page must be contiguous")
-    page = heads * size
-    return (key_pages.data_ptr(), value_pages.data_ptr(), ks[0] if blocks > 1 else page,
-            vs[0] if blocks > 1 else page, blocks, heads, size // per_token, head_dim)
+    if blocks > 1 and ks[0] != vs[0]:
+        raise ValueError("key and value pages must have the same stride")
+    return (key_pages.data_ptr(), value_pages.data_ptr(), ks[0] if blocks > 1 else heads * size,
+            blocks, heads, size // per_token, head_dim)
 
 
 def _rows(key: torch.Tensor, value: torch.Tensor, tokens: int, heads: int, head_dim: int,
@@ -142,7 +143,7 @@ def write(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
     device = key_pages.device
     c = _cache(key_pages, value_pages, key.shape[2])
     tokens = _slots(slots, device)
-    kind, *strides = _rows(key, value, tokens, c[5], c[7], device)
+    kind, *strides = _rows(key, value, tokens, c[4], c[6], device)
     if tokens:
         _call(device, "kvx_q4_write", key.data_ptr(), value.data_ptr(), kind, tokens, *strides,
               slots.data_ptr(), *c)
@@ -161,11 +162,11 @@ def read(key_pages: torch.Tensor, value_pages: torch.Tensor, slots: torch.Tensor
     if out is None:
         if dtype not in _DTYPES:
             raise TypeError(f"rows are read as bfloat16, float16 or float32, not {dtype}")
-        key = torch.empty((tokens, c[5], head_dim), dtype=dtype, device=device)
+        key = torch.empty((tokens, c[4], head_dim), dtype=dtype, device=device)
         value = torch.empty_like(key)
     else:
         key, value = out
-    kind, *strides = _rows(key, value, tokens, c[5], head_dim, device)
+    kind, *strides = _rows(key, value, tokens, c[4], head_dim, device)
     if tokens:
         _call(device, "kvx_q4_read", *c, slots.data_ptr(), tokens, key.data_ptr(),
               value.data_ptr(), kind, *strides)
@@ -215,8 +216,8 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     kind = _DTYPES.get(query.dtype)
     if kind is None or kind == _lib.DTYPE_FP32:
         raise TypeError(f"query must be bfloat16 or float16, got {query.dtype}")
-    if heads == 0 or heads % c[5]:
-        raise ValueError(f"{heads} query heads are no multiple of {c[5]} kv heads")
+    if heads == 0 or heads % c[4]:
+        raise ValueError(f"{heads} query heads are no multiple of {c[4]} kv heads")
     if block_tables.dtype is not torch.int32 or block_tables.dim() != 2:
         raise ValueError("block_tables must be an int32 tensor [batch, width]")
     if seq_lens.dtype is not torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous():
@@ -264,7 +265,7 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     lse = (torch.empty((tokens, heads), dtype=torch.float32, device=device)
            if return_lse else None)
     if tokens and batch:
-        size = _workspace(device, head_dim, rows * (heads // c[5]))
+        size = _workspace(device, head_dim, rows * (heads // c[4]))
         work = torch.empty(size, dtype=torch.uint8, device=device)
         os_ = out.stride()
         _call(device, "kvx_q4_attention", query.data_ptr(), qs[0], qs[1], out.data_ptr(), os_[0],

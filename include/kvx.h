@@ -356,9 +356,9 @@ int kvx_safetensors_meta_json(const char* file_path, char* out,
  * kvx_swap_blocks and kvx_migrate_blocks move it as they move any page.
  *
  * Common arguments: key_pages / value_pages: page 0 of the two tensors, device
- * memory of the current device, 16-byte aligned; *_page_stride: bytes from one
- * page to the next (a multiple of 16, at least one page); num_blocks pages in
- * each; block_size a multiple of 16 (at most 4096); head_dim 64, 128 or 256.
+ * memory of the current device, 16-byte aligned; page_stride: bytes from one page
+ * to the next in both (a multiple of 16, at least one page); num_blocks pages
+ * in each; block_size a multiple of 16 (at most 4096); head_dim 64, 128 or 256.
  * dtype: KVX_DTYPE_*.  Strides of rows are in elements; the elements of one
  * row are contiguous.  Slot s is token s % block_size of block s / block_size.
  * All device pointers; nothing is read back: a slot, block id or length that
@@ -397,14 +397,12 @@ int kvx_q4_write(const void* key, const void* value, int dtype,
                  int64_t num_tokens, int64_t key_token_stride,
                  int64_t key_head_stride, int64_t value_token_stride,
                  int64_t value_head_stride, const int64_t* slots,
-                 void* key_pages, void* value_pages, int64_t key_page_stride,
-                 int64_t value_page_stride, int64_t num_blocks,
-                 int64_t kv_heads, int64_t block_size, int64_t head_dim,
-                 void* stream);
+                 void* key_pages, void* value_pages, int64_t page_stride,
+                 int64_t num_blocks, int64_t kv_heads, int64_t block_size,
+                 int64_t head_dim, void* stream);
 int kvx_q4_read(const void* key_pages, const void* value_pages,
-                int64_t key_page_stride, int64_t value_page_stride,
-                int64_t num_blocks, int64_t kv_heads, int64_t block_size,
-                int64_t head_dim, const int64_t* slots, int64_t num_tokens,
+                int64_t page_stride, int64_t num_blocks, int64_t kv_heads,
+                int64_t block_size, int64_t head_dim, const int64_t* slots, int64_t num_tokens,
                 void* key, void* value, int dtype, int64_t key_token_stride,
                 int64_t key_head_stride, int64_t value_token_stride,
                 int64_t value_head_stride, void* stream);
@@ -415,10 +413,9 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride,
                      int64_t out_token_stride, int64_t out_head_stride,
                      float* lse, int dtype, int64_t num_tokens,
                      int64_t num_heads, const void* key_pages,
-                     const void* value_pages, int64_t key_page_stride,
-                     int64_t value_page_stride, int64_t num_blocks,
-                     int64_t kv_heads, int64_t block_size, int64_t head_dim,
-                     const int32_t* block_tables, int64_t table_stride,
+                     const void* value_pages, int64_t page_stride,
+                     int64_t num_blocks, int64_t kv_heads, int64_t block_size,
+                     int64_t head_dim, const int32_t* block_tables, int64_t table_stride,
                      int64_t table_width, const int32_t* seq_lens,
                      const int32_t* query_starts, int64_t batch, double scale,
                      int64_t window, int64_t sinks, void* workspace,

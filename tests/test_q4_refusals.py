@@ -14,13 +14,13 @@ P = 0x7F0000000000  # a 16-byte aligned address that is never touched
 
 def write(kvx, **kw):
     a = dict(key=P, value=P, dtype=0, tokens=1, kt=1024, kh=128, vt=1024, vh=128, slots=P, kp=P,
-             vp=P, ks=8704, vs=8704, blocks=4, heads=8, block=16, dim=128, stream=None)
+             vp=P, stride=8704, blocks=4, heads=8, block=16, dim=128, stream=None)
     a.update(kw)
     return kvx.kvx_q4_write(*a.values())
 
 
 def read(kvx, **kw):
-    a = dict(kp=P, vp=P, ks=8704, vs=8704, blocks=4, heads=8, block=16, dim=128, slots=P, tokens=1,
+    a = dict(kp=P, vp=P, stride=8704, blocks=4, heads=8, block=16, dim=128, slots=P, tokens=1,
              key=P, value=P, dtype=0, kt=1024, kh=128, vt=1024, vh=128, stream=None)
     a.update(kw)
     return kvx.kvx_q4_read(*a.values())
@@ -28,7 +28,7 @@ def read(kvx, **kw):
 
 def attend(kvx, **kw):
     a = dict(query=P, qt=4096, qh=128, out=P, ot=4096, oh=128, lse=None, dtype=0, tokens=2,
-             num_heads=32, kp=P, vp=P, ks=8704, vs=8704, blocks=4, heads=8, block=16, dim=128,
+             num_heads=32, kp=P, vp=P, stride=8704, blocks=4, heads=8, block=16, dim=128,
              tables=P, table_stride=4, width=4, lens=P, starts=None, batch=2, scale=0.1, window=0,
              sinks=0, work=P, work_bytes=1 << 40, stream=None)
     a.update(kw)
@@ -37,8 +37,8 @@ def attend(kvx, **kw):
 
 CACHE = [
     dict(dim=96), dict(dim=0), dict(block=0), dict(block=24), dict(block=8192), dict(heads=0),
-    dict(heads=1025, ks=1 << 30, vs=1 << 30), dict(blocks=-1), dict(kp=None), dict(vp=None),
-    dict(kp=P + 8), dict(ks=8712), dict(ks=8688), dict(vs=4352),
+    dict(heads=1025, stride=1 << 30), dict(blocks=-1), dict(kp=None), dict(vp=None),
+    dict(kp=P + 8), dict(stride=8712), dict(stride=8688), dict(stride=-16),
 ]
 
 
