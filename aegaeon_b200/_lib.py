@@ -180,6 +180,36 @@ def shim():
     return _shim
 
 
+_q4 = None
+
+
+def q4():
+    """The tensor entry points of the 4-bit cache (``aegaeon_b200/_kvxq4*.so``,
+    built with the library) bound to the functions of ``lib()``; raises if the
+    module is missing."""
+    global _q4
+    if _q4 is not None:
+        return _q4
+    handle = lib()
+    with _lock:
+        if _q4 is None:
+            import torch  # noqa: F401  (its libraries have to be loaded first)
+
+            try:
+                from . import _kvxq4
+            except ImportError as e:
+                raise RuntimeError(
+                    f"the kvx q4 module is missing ({e}); build it with "
+                    "`python -c 'import __graft_entry__ as g; g.build()'` "
+                    "or `python -m aegaeon_b200.build`"
+                ) from e
+            _kvxq4.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in
+                          ("kvx_q4_write", "kvx_q4_read", "kvx_q4_attention",
+                           "kvx_q4_attention_workspace")))
+            _q4 = _kvxq4
+    return _q4
+
+
 def ids_arg(values):
     """Block ids as the call shim takes them: lists and tuples as they are,
     anything else (numpy arrays, tensors, ranges) as an int64 C array."""

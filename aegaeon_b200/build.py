@@ -34,6 +34,8 @@ HEADERS = [
 OUT = os.path.join(HERE, "libkvx.so")
 SHIM_SOURCE = os.path.join(HERE, "csrc", "kvx_pycall.c")
 SHIM_OUT = os.path.join(HERE, "_kvxcall" + sysconfig.get_config_var("EXT_SUFFIX"))
+Q4_SOURCE = os.path.join(HERE, "csrc", "kvx_q4_torch.cpp")
+Q4_OUT = os.path.join(HERE, "_kvxq4" + sysconfig.get_config_var("EXT_SUFFIX"))
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -68,8 +70,35 @@ def build_shim(force: bool = False) -> str:
     return SHIM_OUT
 
 
+def build_q4_module(force: bool = False) -> str:
+    """The tensor entry points of the 4-bit cache (C++ against torch's headers;
+    it reaches libkvx.so through function pointers handed over at import)."""
+    deps = [Q4_SOURCE, os.path.join(ROOT, "include", "kvx.h")]
+    if (not force and os.path.exists(Q4_OUT)
+            and all(os.path.getmtime(p) <= os.path.getmtime(Q4_OUT) for p in deps)):
+        return Q4_OUT
+    import torch
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    home = os.path.dirname(torch.__file__)
+    includes = [sysconfig.get_paths()["include"], cuda, os.path.join(home, "include"),
+                os.path.join(home, "include", "torch", "csrc", "api", "include")]
+    lib = os.path.join(home, "lib")
+    cmd = [cxx, "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-isystem{p}" for p in includes), Q4_SOURCE, f"-L{lib}", "-ltorch_python",
+           "-ltorch_cpu", "-lc10_cuda", "-lc10", "-o", Q4_OUT + ".tmp"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cxx} failed ({res.returncode}):\n{res.stderr}\n{res.stdout}")
+    os.replace(Q4_OUT + ".tmp", Q4_OUT)
+    return Q4_OUT
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     build_shim(force)
+    build_q4_module(force)
     if not force and up_to_date():
         return OUT
     cmd = [

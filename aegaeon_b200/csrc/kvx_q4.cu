@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -96,10 +97,14 @@ int run_rows(bool write, RowArgs& a, int dtype, int64_t num_tokens, int64_t head
   for (const Rows& r : a.rows)
     if (!aligned(r.base, element_size(dtype)))
       return fail(KVX_ERR_INVALID_ARGUMENT, "rows are not aligned to their type");
-  a.num_rows = num_tokens * a.cache.kv_heads;
+  const int64_t num_rows = num_tokens * a.cache.kv_heads;
+  if (num_tokens > INT32_MAX || num_rows > INT32_MAX)
+    return fail(KVX_ERR_INVALID_ARGUMENT, "too many tokens in one call");
+  a.num_rows = uint32_t(num_rows);
+  a.by_heads = Divisor::of(uint32_t(a.cache.kv_heads));
+  a.by_block = Divisor::of(uint32_t(a.cache.block_size));
   const int64_t per_block = kRowThreads / (head_dim / 16);
-  const int64_t grid = (a.num_rows + per_block - 1) / per_block;
-  if (grid > INT32_MAX) return fail(KVX_ERR_INVALID_ARGUMENT, "too many tokens in one call");
+  const int64_t grid = (num_rows + per_block - 1) / per_block;
   const bool vec = rows_vec(a.rows[0], dtype) && rows_vec(a.rows[1], dtype);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == kBf16) launch_rows<__nv_bfloat16>(write, vec, int(head_dim), a, unsigned(grid), s);
@@ -124,10 +129,9 @@ int resident(int rows, int64_t head_dim, int sms) {
   return sms * (rows <= 16 && head_dim <= 128 ? 2 : 1);
 }
 
-int sm_count(int* sms) {
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
+int sm_count(int* sms, int* device) {
+  cudaError_t e = cudaGetDevice(device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *device);
   return e == cudaSuccess ? KVX_OK : cuda_fail("cudaDeviceGetAttribute", e);
 }
 
@@ -140,11 +144,17 @@ uint64_t workspace_of(int rows, int64_t head_dim, int sms) {
 }
 
 template <typename T, int D, int NT>
-int launch_attention(const AttnArgs& a, int grid, int64_t items, cudaStream_t s) {
+int launch_attention(const AttnArgs& a, int grid, int64_t items, int device, cudaStream_t s) {
   constexpr int shared = Shape<D>::kShared;
-  cudaError_t e = cudaFuncSetAttribute(q4_attend<T, D, NT>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-  if (e != cudaSuccess) return cuda_fail("cudaFuncSetAttribute", e);
+  static std::atomic<uint64_t> allowed{0};  // devices that know the shared-memory size
+  cudaError_t e = cudaSuccess;
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(q4_attend<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             shared);
+    if (e != cudaSuccess) return cuda_fail("cudaFuncSetAttribute", e);
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   q4_attend<T, D, NT><<<grid, kThreads, shared, s>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail("q4_attend", e);
@@ -169,19 +179,19 @@ int launch_attention(const AttnArgs& a, int grid, int64_t items, cudaStream_t s)
 
 template <typename T>
 int launch_attention(const AttnArgs& a, int64_t head_dim, int rows, int grid, int64_t items,
-                     cudaStream_t s) {
+                     int device, cudaStream_t s) {
   if (head_dim == 64) {
-    if (rows == 8) return launch_attention<T, 64, 1>(a, grid, items, s);
-    if (rows == 16) return launch_attention<T, 64, 2>(a, grid, items, s);
-    return launch_attention<T, 64, 4>(a, grid, items, s);
+    if (rows == 8) return launch_attention<T, 64, 1>(a, grid, items, device, s);
+    if (rows == 16) return launch_attention<T, 64, 2>(a, grid, items, device, s);
+    return launch_attention<T, 64, 4>(a, grid, items, device, s);
   }
   if (head_dim == 128) {
-    if (rows == 8) return launch_attention<T, 128, 1>(a, grid, items, s);
-    if (rows == 16) return launch_attention<T, 128, 2>(a, grid, items, s);
-    return launch_attention<T, 128, 4>(a, grid, items, s);
+    if (rows == 8) return launch_attention<T, 128, 1>(a, grid, items, device, s);
+    if (rows == 16) return launch_attention<T, 128, 2>(a, grid, items, device, s);
+    return launch_attention<T, 128, 4>(a, grid, items, device, s);
   }
-  if (rows == 8) return launch_attention<T, 256, 1>(a, grid, items, s);
-  return launch_attention<T, 256, 2>(a, grid, items, s);
+  if (rows == 8) return launch_attention<T, 256, 1>(a, grid, items, device, s);
+  return launch_attention<T, 256, 2>(a, grid, items, device, s);
 }
 
 }  // namespace
@@ -242,8 +252,8 @@ int kvx_q4_attention_workspace(int64_t head_dim, int64_t rows_per_sequence, uint
   if (!bytes_out) return fail(KVX_ERR_INVALID_ARGUMENT, "null bytes_out");
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return fail(KVX_ERR_INVALID_ARGUMENT, "head_dim must be 64, 128 or 256");
-  int sms = 0;
-  const int rc = sm_count(&sms);
+  int sms = 0, device = 0;
+  const int rc = sm_count(&sms, &device);
   if (rc) return rc;
   *bytes_out = workspace_of(tile_rows(rows_per_sequence, head_dim), head_dim, sms);
   return KVX_OK;
@@ -285,8 +295,8 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
     return fail(KVX_ERR_INVALID_ARGUMENT, "request too large for one call");
   const int64_t queries = query_starts ? num_tokens : num_tokens / batch;
   const int rows = tile_rows(queries * group, head_dim);
-  int sms = 0;
-  rc = sm_count(&sms);
+  int sms = 0, device = 0;
+  rc = sm_count(&sms, &device);
   if (rc) return rc;
   if (!workspace || workspace_bytes < workspace_of(rows, head_dim, sms))
     return fail(KVX_ERR_INVALID_ARGUMENT,
@@ -331,8 +341,8 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == kBf16 ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), items, s)
-                        : launch_attention<__half>(a, head_dim, rows, int(grid), items, s);
+  return dtype == kBf16 ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), items, device, s)
+                        : launch_attention<__half>(a, head_dim, rows, int(grid), items, device, s);
 }
 
 }  // extern "C"

@@ -309,24 +309,6 @@ __device__ __forceinline__ float2 half2_at(uint32_t x) {
   __builtin_memcpy(&h, &x, 4);
   return __half22float2(h);
 }
-// Two additions, or two fused multiply-adds, in one instruction.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{.reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
-      " mov.b64 {%0, %1}, x;}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{.reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-
 // Shared-memory addresses of a lane's parts of a stage (the stage's base in).
 struct LaneAddress {
   uint32_t k;       // its 16 bytes (D = 64: 8) of K row g

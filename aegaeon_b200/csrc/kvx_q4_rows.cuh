@@ -42,12 +42,40 @@ struct Rows {
   int64_t head_stride;
 };
 
+// Division of 32-bit numbers by a divisor known at launch (Granlund and
+// Montgomery, "Division by invariant integers using multiplication").
+struct Divisor {
+  uint32_t d, m, s1, s2;
+  __host__ static Divisor of(uint32_t d) {
+    uint32_t l = 0;
+    while (l < 32 && (uint64_t(1) << l) < d) ++l;
+    const uint64_t m = ((uint64_t(1) << 32) * ((uint64_t(1) << l) - d)) / d + 1;
+    return Divisor{d, uint32_t(m), l < 1 ? l : 1u, l > 1 ? l - 1 : 0u};
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    const uint32_t t = __umulhi(m, n);
+    return (t + ((n - t) >> s1)) >> s2;
+  }
+};
+
 struct RowArgs {
   Cache cache;
   Rows rows[2];
   const int64_t* slots;
-  int64_t num_rows;    // tokens * kv_heads
+  uint32_t num_rows;   // tokens * kv_heads
+  Divisor by_heads, by_block;
 };
+
+// Block of a slot and token in the block.
+__device__ __forceinline__ int64_t block_of(const RowArgs& a, int64_t slot, int* within) {
+  if (uint64_t(slot) < (uint64_t(1) << 32)) {
+    const uint32_t block = a.by_block.quotient(uint32_t(slot));
+    *within = int(uint32_t(slot) - block * a.by_block.d);
+    return block;
+  }
+  *within = int(slot % a.cache.block_size);
+  return slot / a.cache.block_size;
+}
 
 template <typename T>
 struct Pair;
@@ -123,18 +151,76 @@ __device__ __forceinline__ int64_t head_offset(const Cache& c, int64_t block, in
   return block * c.stride + int64_t(head) * c.head_bytes;
 }
 
-// Code of x in [0, 15]: rint((x - zero) / scale), ties to even, in real
-// arithmetic.  The product with the reciprocal is off by at most 3 * 2^-24 of
-// a quotient below 16 (three roundings), under 3e-6; only where the quotient
-// lies within 1e-5 of a border between two codes does the 64-bit division
-// decide, which the 16-bit types' differences enter exactly.
-__device__ __forceinline__ uint32_t code_of(float x, float zero, float scale, float inv) {
-  const float t = fminf(fmaxf((x - zero) * inv, 0.f), 15.f);
-  const float r = t + 12582912.f;  // 1.5 * 2^23: the sum's low bits are rint(t)
-  uint32_t c = __float_as_uint(r) & 15u;
-  if (fabsf(t - (r - 12582912.f)) > 0.49999f)
-    c = uint32_t(fmin(fmax(rint((double(x) - double(zero)) / double(scale)), 0.0), 15.0));
+// Two additions, or two fused multiply-adds, in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{.reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// The code next to a border, decided exactly: `c` is the nearest code or the one
+// beside it.  d + e = x - zero without an error (two-sum), c * scale has at most
+// 15 bits, and the difference of d to it, about scale / 2, is representable, as
+// is its difference to scale / 2: only the last sum rounds, which keeps its sign.
+__device__ __forceinline__ uint32_t settle(float x, float zero, float scale, uint32_t c) {
+  const float d = x - zero, near = x - d;
+  const float e = (x - (d + near)) + (near - zero);
+  const float r = fmaf(-float(c), scale, d), half = 0.5f * scale;
+  const float above = (r - half) + e, below = (r + half) + e;
+  if (above > 0.f || (above == 0.f && (c & 1u))) return min(c + 1u, 15u);
+  if (below < 0.f || (below == 0.f && (c & 1u))) return c ? c - 1u : 0u;
   return c;
+}
+
+// Codes of 16 values, two words of eight: rint((x - zero) / scale) in [0, 15],
+// ties to even, in real arithmetic.
+//
+// u = (x - zero) / (15 scale), clamped to [0, 1], carries three roundings, so 15 u is
+// off by less than 15 * 3 * 2^-24 < 3e-6.  15 u + 1.5 * 2^23 is rounded once, to the
+// nearest integer, which then stands in the sum's low bits.  The result can
+// differ from the definition's only where what is left over is within 1e-5 of
+// half a step; a thread that has such a value settles its 16 again (16-bit
+// values meet exact ties often: about one in three thousand of them).
+template <typename T>
+__device__ __forceinline__ uint2 codes_of(const T (&x)[16], float zero, float scale) {
+  constexpr float kMagic = 12582912.f;
+  const float inverse = 1.f / (15.f * scale);
+  uint32_t w[2] = {0u, 0u};
+  float far = 0.f;  // largest distance from a code's value
+#pragma unroll
+  for (int i = 14; i >= 0; i -= 2) {
+    const float2 d = add2(make_float2(to_float(x[i]), to_float(x[i + 1])), both(-zero));
+    const float2 u = make_float2(__saturatef(d.x * inverse), __saturatef(d.y * inverse));
+    const float2 r = fma2(u, both(15.f), both(kMagic));
+    const float2 left = fma2(add2(r, both(-kMagic)), both(-scale), d);
+    far = fmaxf(far, fmaxf(fabsf(left.x), fabsf(left.y)));
+    w[i / 8] = (w[i / 8] * 16u + __float_as_uint(r.y)) * 16u + __float_as_uint(r.x);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) w[h] -= 0x3F400000u;  // 0x4B400000 * 0x11111111
+  if (far > 0.49999f * scale) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v |= settle(to_float(x[8 * h + i]), zero, scale, (w[h] >> (4 * i)) & 15u) << (4 * i);
+      w[h] = v;
+    }
+  }
+  return make_uint2(w[0], w[1]);
 }
 
 // Quantise.  D/16 lanes share a row, 16 elements each; every thread takes the
@@ -142,23 +228,16 @@ __device__ __forceinline__ uint32_t code_of(float x, float zero, float scale, fl
 template <typename T, int D, bool kVec>
 __global__ void __launch_bounds__(kRowThreads) q4_write(const RowArgs a) {
   constexpr int kLanes = D / 16;
-  const int64_t row = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) / kLanes;
+  const uint32_t row = blockIdx.x * (kRowThreads / kLanes) + threadIdx.x / kLanes;
   const int lane = threadIdx.x % kLanes;
   const bool inside = row < a.num_rows;
-  const int64_t token = inside ? row / a.cache.kv_heads : 0;
-  const int head = inside ? int(row % a.cache.kv_heads) : 0;
+  const uint32_t token = inside ? a.by_heads.quotient(row) : 0u;
+  const int head = inside ? int(row - token * a.by_heads.d) : 0;
   const int64_t slot = inside ? a.slots[token] : -1;
-  const int64_t block = slot / a.cache.block_size;
-  bool live = inside && slot >= 0;
-  if (live && block >= a.cache.num_blocks) {
-    live = false;
-    if (lane == 0) atomicExch(&g_q4_status, 5 /* KVX_ERR_BLOCK_ID */);
-  }
-  const int within = int(slot % a.cache.block_size);
   T x[2][16];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    if (live) {
+  for (int s = 0; s < 2; ++s) {  // whatever the slot, so that no load waits for it
+    if (inside) {
       load16<T, kVec>(static_cast<const T*>(a.rows[s].base) + token * a.rows[s].token_stride +
                           head * a.rows[s].head_stride + lane * 16,
                       x[s]);
@@ -166,6 +245,13 @@ __global__ void __launch_bounds__(kRowThreads) q4_write(const RowArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[s][i] = from_float<T>(0.f);
     }
+  }
+  int within;
+  const int64_t block = block_of(a, slot, &within);
+  bool live = slot >= 0;
+  if (live && block >= a.cache.num_blocks) {
+    live = false;
+    if (lane == 0) atomicExch(&g_q4_status, 5 /* KVX_ERR_BLOCK_ID */);
   }
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
@@ -203,16 +289,11 @@ __global__ void __launch_bounds__(kRowThreads) q4_write(const RowArgs a) {
     const __half scale_h = __float2half_rn((hi - lo) / 15.f);
     const __half zero_h = __float2half_rn(lo);
     const float scale = __half2float(scale_h), zero = __half2float(zero_h);
-    uint32_t w[2] = {0u, 0u};
-    if (finite && scale > 0.f) {
-      const float inv = 1.f / scale;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        w[i / 8] |= code_of(to_float(x[s][i]), zero, scale, inv) << (4 * (i % 8));
-    }
+    uint2 w = make_uint2(0u, 0u);
+    if (finite && scale > 0.f) w = codes_of(x[s], zero, scale);
     if (live) {
       uint8_t* page = a.cache.pages[s] + head_offset(a.cache, block, head);
-      *reinterpret_cast<uint2*>(page + within * (D / 2) + lane * 8) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(page + within * (D / 2) + lane * 8) = w;
       if (lane == 0)
         *reinterpret_cast<__half2*>(page + a.cache.block_size * (D / 2) + within * 4) =
             finite ? __halves2half2(scale_h, zero_h)
@@ -226,19 +307,19 @@ __global__ void __launch_bounds__(kRowThreads) q4_write(const RowArgs a) {
 template <typename T, int D, bool kVec>
 __global__ void __launch_bounds__(kRowThreads) q4_read(const RowArgs a) {
   constexpr int kLanes = D / 16;
-  const int64_t row = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) / kLanes;
+  const uint32_t row = blockIdx.x * (kRowThreads / kLanes) + threadIdx.x / kLanes;
   const int lane = threadIdx.x % kLanes;
   if (row >= a.num_rows) return;
-  const int64_t token = row / a.cache.kv_heads;
-  const int head = int(row % a.cache.kv_heads);
+  const uint32_t token = a.by_heads.quotient(row);
+  const int head = int(row - token * a.by_heads.d);
   const int64_t slot = a.slots[token];
-  const int64_t block = slot / a.cache.block_size;
+  int within;
+  const int64_t block = block_of(a, slot, &within);
   bool live = slot >= 0;
   if (live && block >= a.cache.num_blocks) {
     live = false;
     if (lane == 0) atomicExch(&g_q4_status, 5 /* KVX_ERR_BLOCK_ID */);
   }
-  const int within = int(slot % a.cache.block_size);
   uint2 w[2] = {};
   __half2 p[2] = {};
   if (live) {
@@ -255,8 +336,9 @@ __global__ void __launch_bounds__(kRowThreads) q4_read(const RowArgs a) {
     T x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const uint32_t c = ((i < 8 ? w[s].x : w[s].y) >> (4 * (i % 8))) & 15u;
-      x[i] = from_float<T>(fmaf(float(c), scale, zero));
+      // The code in the low bits of 2^23 is that number more.
+      const uint32_t c = (((i < 8 ? w[s].x : w[s].y) >> (4 * (i % 8))) & 15u) | 0x4B000000u;
+      x[i] = from_float<T>(fmaf(__uint_as_float(c) - 8388608.f, scale, zero));
     }
     store16<T, kVec>(static_cast<T*>(a.rows[s].base) + token * a.rows[s].token_stride +
                          head * a.rows[s].head_stride + lane * 16,
