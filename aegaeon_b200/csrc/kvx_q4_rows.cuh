@@ -168,6 +168,19 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float max_abs(float m, float a, float b) {  // max(m, |a|, |b|)
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // The code next to a border, decided exactly: `c` is the nearest code or the one
@@ -187,37 +200,45 @@ __device__ __forceinline__ uint32_t settle(float x, float zero, float scale, uin
 // Codes of 16 values, two words of eight: rint((x - zero) / scale) in [0, 15],
 // ties to even, in real arithmetic.
 //
-// u = (x - zero) / (15 scale), clamped to [0, 1], carries three roundings, so 15 u is
-// off by less than 15 * 3 * 2^-24 < 3e-6.  15 u + 1.5 * 2^23 is rounded once, to the
-// nearest integer, which then stands in the sum's low bits.  The result can
-// differ from the definition's only where what is left over is within 1e-5 of
-// half a step; a thread that has such a value settles its 16 again (16-bit
-// values meet exact ties often: about one in three thousand of them).
+// q = (x - zero) * (1 / scale) carries the roundings of the difference and the
+// product and the reciprocal's 2 ulp, below 16 * 4 * 2^-23 < 8e-6 in all.
+// q + 1.5 * 2^23 is rounded once, to the nearest integer, which then stands in
+// the sum's low bits.  The result can differ from the definition's only where
+// what is left over is within 1e-5 of half a step; a thread that has such a value
+// settles its 16 again (16-bit values meet exact ties often: about one in three
+// thousand of them).  So does a row with clamped values, or whose zero is so far
+// from 0 that its rounding to fp16 may move values beyond the codes' ends.
 template <typename T>
-__device__ __forceinline__ uint2 codes_of(const T (&x)[16], float zero, float scale) {
+__device__ __forceinline__ uint2 codes_of(const T (&x)[16], float zero, float scale,
+                                          bool clamped) {
   constexpr float kMagic = 12582912.f;
-  const float inverse = 1.f / (15.f * scale);
+  float inverse;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
   uint32_t w[2] = {0u, 0u};
   float far = 0.f;  // largest distance from a code's value
 #pragma unroll
   for (int i = 14; i >= 0; i -= 2) {
     const float2 d = add2(make_float2(to_float(x[i]), to_float(x[i + 1])), both(-zero));
-    const float2 u = make_float2(__saturatef(d.x * inverse), __saturatef(d.y * inverse));
-    const float2 r = fma2(u, both(15.f), both(kMagic));
+    const float2 r = add2(mul2(d, both(inverse)), both(kMagic));
     const float2 left = fma2(add2(r, both(-kMagic)), both(-scale), d);
-    far = fmaxf(far, fmaxf(fabsf(left.x), fabsf(left.y)));
+    far = max_abs(far, left.x, left.y);
     w[i / 8] = (w[i / 8] * 16u + __float_as_uint(r.y)) * 16u + __float_as_uint(r.x);
   }
 #pragma unroll
   for (int h = 0; h < 2; ++h) w[h] -= 0x3F400000u;  // 0x4B400000 * 0x11111111
-  if (far > 0.49999f * scale) {
+  // zero is off its value by at most 2^-11 |zero|, scale by 2^-11 of itself: below
+  // this bound every quotient stays in (-1/2, 15 1/2).
+  const bool beyond = clamped || fabsf(zero) > 900.f * scale || scale < 6.2e-5f;
+  const float border = 0.49999f * scale;
+  if (beyond || far > border) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t v = 0u;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v |= settle(to_float(x[8 * h + i]), zero, scale, (w[h] >> (4 * i)) & 15u) << (4 * i);
-      w[h] = v;
+    for (int i = 0; i < 16; ++i) {
+      const float y = to_float(x[i]);
+      const uint32_t was = (w[i / 8] >> (4 * (i % 8))) & 15u;
+      if (!beyond && fabsf(fmaf(-float(was), scale, y - zero)) <= border) continue;
+      uint32_t c = was;
+      if (beyond) c = uint32_t(fminf(fmaxf((y - zero) / scale, 0.f), 15.f) + 0.5f);
+      w[i / 8] ^= (was ^ settle(y, zero, scale, c)) << (4 * (i % 8));
     }
   }
   return make_uint2(w[0], w[1]);
@@ -284,13 +305,14 @@ __global__ void __launch_bounds__(kRowThreads) q4_write(const RowArgs a) {
     }
     // A row with a NaN or an infinity reads back as NaN: it is marked, not hidden.
     const bool finite = fabsf(lo) <= 3.402823466e38f && fabsf(hi) <= 3.402823466e38f;
+    const bool clamped = fmaxf(fabsf(lo), fabsf(hi)) > kLimit;
     lo = fminf(fmaxf(lo, -kLimit), kLimit);
     hi = fminf(fmaxf(hi, -kLimit), kLimit);
     const __half scale_h = __float2half_rn((hi - lo) / 15.f);
     const __half zero_h = __float2half_rn(lo);
     const float scale = __half2float(scale_h), zero = __half2float(zero_h);
     uint2 w = make_uint2(0u, 0u);
-    if (finite && scale > 0.f) w = codes_of(x[s], zero, scale);
+    if (finite && scale > 0.f) w = codes_of(x[s], zero, scale, clamped);
     if (live) {
       uint8_t* page = a.cache.pages[s] + head_offset(a.cache, block, head);
       *reinterpret_cast<uint2*>(page + within * (D / 2) + lane * 8) = w;
