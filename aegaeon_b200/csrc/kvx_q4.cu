@@ -125,9 +125,7 @@ int tile_rows(int64_t rows, int64_t head_dim) {
 }
 
 // CTAs that are resident on the device at once.
-int resident(int rows, int64_t head_dim, int sms) {
-  return sms * (rows <= 16 && head_dim <= 128 ? 2 : 1);
-}
+int resident(int sms) { return 2 * sms; }
 
 int sm_count(int* sms, int* device) {
   cudaError_t e = cudaGetDevice(device);
@@ -140,7 +138,7 @@ int sm_count(int* sms, int* device) {
 constexpr int64_t kJoinByRow = 64;
 
 uint64_t workspace_of(int rows, int64_t head_dim, int sms) {
-  return 2ull * resident(rows, head_dim, sms) * rows * (4 * head_dim + 8);
+  return 2ull * resident(sms) * rows * (4 * head_dim + 8);
 }
 
 template <typename T, int D, int NT>
@@ -332,12 +330,12 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   const int64_t tiles = query_starts ? num_tokens * group / rows + batch
                                      : batch * ((queries * group + rows - 1) / rows);
   const int64_t units = std::max<int64_t>(table_width * a.upp, 1);
-  int64_t grid = resident(rows, head_dim, sms);
+  int64_t grid = resident(sms);
   const int64_t items = tiles * kv_heads;
   const double bound =
       double(items) * double(units + kItemUnits) / double(kMinUnits + kItemUnits);
   if (bound < double(grid)) grid = std::max<int64_t>(1, int64_t(std::ceil(bound)));
-  const int64_t pieces = 2ll * resident(rows, head_dim, sms) * rows;
+  const int64_t pieces = 2ll * resident(sms) * rows;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -19,13 +19,12 @@
 namespace kvx {
 namespace q4 {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 3;       // pairs of units in flight or in use, per warp
+constexpr int kStages = 3;       // steps in flight or in use, per warp
 constexpr int kNoWindow = 1 << 30;
-// Fewest 16-token units a CTA takes: two for each warp.  Fewer make the join
-// the larger part of the work.
-constexpr int kMinUnits = 2 * kWarps;
+// Fewest 16-token units a CTA takes: four for each warp, a whole step.
+constexpr int kMinUnits = 4 * kWarps;
 // What an item (a tile of query rows with one kv head) costs besides its units,
 // in units: its queries, its first block ids and the join of the warps.
 constexpr int kItemUnits = 16;
@@ -176,13 +175,16 @@ constexpr uint32_t kOdd = 0x00f000f0u;   // nibbles 1 and 5: code * 2^-20
 template <int D>
 struct Shape {
   static constexpr int kUnit = 8 * D;           // bytes of codes of 16 tokens
-  static constexpr int kStage = 4 * kUnit + 256;  // K and V of two units, (scale, zero) of each
+  // Units of a step, which a warp takes at a time.  With four, what a step costs
+  // besides its units (addresses, the vote on the reference point) is a tenth.
+  static constexpr int kUnits = D == 256 ? 2 : 4;
+  static constexpr int kParams = kUnits * 64;   // (scale, zero) of the units' tokens, one tensor
+  static constexpr int kStage = kUnits * 2 * kUnit + 2 * kParams;
   static constexpr int kWarpBytes = kStages * kStage;
   static constexpr int kRing = kWarps * kWarpBytes;
   static constexpr int kJoin = kWarps * 8 * (D + 4) * 4;
   static constexpr int kShared = kRing > kJoin ? kRing : kJoin;
   static constexpr int kKeyWords = D / 32;      // code words of a thread for one token of K
-  static constexpr int kValueWords = D / 64;    // ... for one token of V
 };
 
 // First dimension of code word w of quad lane j in a K row.  At D = 256 the
@@ -212,6 +214,7 @@ template <typename T, int D, int NT>
 __device__ __forceinline__ void load_queries(const AttnArgs& a, const Seq& s, int row0, int rows,
                                              int head, TileShared<D, NT>& sh) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
+  static_assert(NT <= kWarps, "a warp for each eight rows");
   if (warp >= NT) return;
   const int r = warp * 8 + g;
   const bool real = r < rows;
@@ -279,7 +282,8 @@ template <int D, int NT>
 struct WarpState {
   float o[NT][D / 16][4];  // sum of p * s * C * code, dimensions as in value_dim()
   float ps[NT][4];         // sum of the same weights as the matrix instruction saw them
-  float2 m[NT], l[NT];     // reference point and sum of the weights, by column
+  float2 m[NT], l[NT];     // minus the reference point, sum of the weights, by column
+  float2 limit[NT];        // raw score that moves the reference point
   float z[NT][2];          // sum of p * (zero + 7.5 scale)
   float c;                 // C: power of two on the V scales, so that weights suit fp16
 };
@@ -323,14 +327,14 @@ struct LaneAddress {
 template <int D>
 __device__ __forceinline__ LaneAddress lane_address(uint32_t base, int g, int j) {
   LaneAddress a;
-  const uint32_t values = base + 2 * Shape<D>::kUnit;
+  const uint32_t values = base + Shape<D>::kUnits * Shape<D>::kUnit;
   const uint32_t swizzle = 32u * (D == 64 ? (j >> 1) & 1 : j);
   const uint32_t v = uint32_t(D * j + (D / 16) * g) ^ swizzle;  // row 2j has D/2 bytes
   a.v0 = values + v;
   a.v1 = values + (v ^ (D / 2));
   a.k = base + (D / 2) * g + (D == 256 ? 16 * (j ^ (4 * (g & 1))) : (D / 8) * j);
   a.k_far = D == 256 ? base + 128 * g + (16 * (j ^ (4 * (g & 1))) ^ 64) : 0u;
-  a.p = base + 4 * Shape<D>::kUnit + 4 * g;
+  a.p = base + 2 * Shape<D>::kUnits * Shape<D>::kUnit + 4 * g;
   return a;
 }
 
@@ -426,39 +430,56 @@ struct Columns {
   int pos[NT][2];
 };
 
-// kAb units from unit U of the stage on: scores, softmax, products.  `number` are the
-// units' numbers in the sequence, -1 for one that is not there.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// f(Index<0>), ..., f(Index<N - 1>): an index known at compile time.
+template <int I>
+struct Index {
+  static constexpr int value = I;
+};
+template <int N, class F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(Index<N - 1>{});
+  }
+}
+
+// kAb units from unit U of the stage on: scores, softmax, products.  `number`
+// gives the units' numbers in the sequence, -1 for one that is not there.
 template <int D, int NT, int U, int kAb, bool kMasked>
 __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared<D, NT>& sh,
                                              const uint2* qreg, const LaneAddress& at,
-                                             const int (&number)[2], const Columns<NT>& col,
+                                             const int* number, const Columns<NT>& col,
                                              const Span& v, WarpState<D, NT>& st) {
   const int lane = threadIdx.x % 32, g = lane / 4;
   float x[kAb][NT][4];
-  unit_scores<D, NT, U>(at, sh, qreg, x[0]);
-  if constexpr (kAb == 2) unit_scores<D, NT, 1>(at, sh, qreg, x[1]);
   // (scale, zero) of tokens g and g + 8 of each unit: K, then V.
   uint32_t kp[kAb][2], vp[kAb][2];
-  kp[0][0] = lds32<64 * U>(at.p), kp[0][1] = lds32<64 * U + 32>(at.p);
-  vp[0][0] = lds32<128 + 64 * U>(at.p), vp[0][1] = lds32<128 + 64 * U + 32>(at.p);
-  if constexpr (kAb == 2) {
-    kp[1][0] = lds32<64>(at.p), kp[1][1] = lds32<96>(at.p);
-    vp[1][0] = lds32<192>(at.p), vp[1][1] = lds32<224>(at.p);
-  }
-  float top[NT][2], vs[kAb][2], vz[kAb][2], most = 0.f;
+  each<kAb>([&](auto index) {
+    constexpr int u = decltype(index)::value, at_u = 64 * (U + u);
+    kp[u][0] = lds32<at_u>(at.p), kp[u][1] = lds32<at_u + 32>(at.p);
+    vp[u][0] = lds32<Shape<D>::kParams + at_u>(at.p);
+    vp[u][1] = lds32<Shape<D>::kParams + at_u + 32>(at.p);
+    unit_scores<D, NT, U + u>(at, sh, qreg, x[u]);
+  });
+  float vs[kAb][2], vz[kAb][2], most = 0.f;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = kNegInf;
-#pragma unroll
-  for (int u = 0; u < kAb; ++u)
+  for (int u = 0; u < kAb; ++u) {
+    float part[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float2 k = half2_at(kp[u][r]), w = half2_at(vp[u][r]);
-      vs[u][r] = w.x;
+      vs[u][r] = part[r] = w.x;
       vz[u][r] = fmaf(7.5f, w.x, w.y);
-      const int unit = number[U + u], t = unit * 16 + g + 8 * r;
+      const int unit = kMasked ? number[u] : 0, t = unit * 16 + g + 8 * r;
       // Only of tokens that some row sees: what lies behind a sequence may be anything.
-      if (!kMasked || (unit >= 0 && t <= v.p_hi && (t > v.p_lo - a.window || t < a.sinks)))
-        most = fmaxf(most, fabsf(w.x));
+      if (kMasked && !(unit >= 0 && t <= v.p_hi && (t > v.p_lo - a.window || t < a.sinks)))
+        part[r] = 0.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -470,17 +491,23 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
             const bool seen = unit >= 0 && t <= p && (t > p - a.window || t < a.sinks);
             y = seen ? y : kNegInf;
           }
-          top[n][c] = fmaxf(top[n][c], y);
         }
     }
+    most = max_abs(most, part[0], part[1]);
+  }
   // Move the reference point where a score passes it by 2^8, or the weights
   // would leave fp16.  The factors are positive, so raw scores have the order.
-  bool move = !(most * st.c <= 64.f) || st.c == 0.f;
+  float top[NT][2];
+  bool move = !(most * st.c <= 64.f);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    top[n][0] *= col.factor[n].x;
-    top[n][1] *= col.factor[n].y;
-    move |= top[n][0] > st.m[n].x + 8.f || top[n][1] > st.m[n].y + 8.f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      top[n][c] = fmaxf(x[0][n][c], x[0][n][2 + c]);
+#pragma unroll
+      for (int u = 1; u < kAb; ++u) top[n][c] = max3(top[n][c], x[u][n][c], x[u][n][2 + c]);
+    }
+    move |= top[n][0] > st.limit[n].x || top[n][1] > st.limit[n].y;
   }
   if (__any_sync(~0u, move)) {
 #pragma unroll
@@ -498,12 +525,14 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
       float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        const float factor = c ? col.factor[n].y : col.factor[n].x;
         float& m = c ? st.m[n].y : st.m[n].x;
-        float t = fmaxf(top[n][c], m);
+        float t = fmaxf(top[n][c] * factor, -m);
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
-        f[c] = t == kNegInf ? 1.f : ex2(m - t);
-        m = t;
+        f[c] = t == kNegInf ? 1.f : ex2(-m - t);
+        m = -t;
+        (c ? st.limit[n].y : st.limit[n].x) = (t + 8.f) / factor;
       }
       st.l[n].x *= f[0], st.l[n].y *= f[1];
       st.z[n][0] *= f[0], st.z[n][1] *= f[1];
@@ -525,11 +554,10 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
       for (int n = 0; n < NT; ++n) {
         float2 m = st.m[n];
         if (kMasked) {
-          m.x = m.x == kNegInf ? 0.f : m.x;
-          m.y = m.y == kNegInf ? 0.f : m.y;
+          m.x = m.x == -kNegInf ? 0.f : m.x;
+          m.y = m.y == -kNegInf ? 0.f : m.y;
         }
-        float2 p = fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]), col.factor[n],
-                        make_float2(-m.x, -m.y));
+        float2 p = fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]), col.factor[n], m);
         p.x = ex2(p.x), p.y = ex2(p.y);
         st.l[n] = add2(st.l[n], p);
         float y[2] = {p.x * weight, p.y * weight};
@@ -545,8 +573,30 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
         b[u][n][r] = transpose8x8(bits);
       }
     }
-  unit_values<D, NT, U>(at, b[0], st);
-  if constexpr (kAb == 2) unit_values<D, NT, 1>(at, b[1], st);
+  each<kAb>([&](auto index) {
+    constexpr int u = decltype(index)::value;
+    unit_values<D, NT, U + u>(at, b[u], st);
+  });
+}
+
+// The units of a step, as many at a time as the registers hold.
+template <int D, int NT, bool kMasked>
+__device__ __forceinline__ void attend_step(const AttnArgs& a, const TileShared<D, NT>& sh,
+                                            const uint2* qreg, const LaneAddress& at,
+                                            const int* number, const Columns<NT>& col,
+                                            const Span& v, WarpState<D, NT>& st) {
+  constexpr int kAll = Shape<D>::kUnits;
+  constexpr int kAb = NT == 4 ? 1 : NT == 2 || D == 256 || kMasked ? 2 : 4;
+  each<kAll / kAb>([&](auto index) {
+    constexpr int kFirst = decltype(index)::value * kAb;
+    if constexpr (kMasked) {  // units behind the last are not there
+      bool any = false;
+#pragma unroll
+      for (int u = 0; u < kAb; ++u) any |= number[kFirst + u] >= 0;
+      if (!any) return;
+    }
+    attend_units<D, NT, kFirst, kAb, kMasked>(a, sh, qreg, at, number + kFirst, col, v, st);
+  });
 }
 
 // Four dimensions of one row's result: sum / l and log-sum-exp; zeros and -inf
@@ -585,12 +635,13 @@ __device__ __forceinline__ void attend_segment(const AttnArgs& a, TileShared<D, 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
   uint8_t* mine = ring + warp * S::kWarpBytes;
   const uint32_t mine_s = uint32_t(__cvta_generic_to_shared(mine));
-  const int pairs = (u1 - u0 + 1) / 2;
-  const int steps = pairs > warp ? (pairs - warp + kWarps - 1) / kWarps : 0;
+  constexpr int kU = S::kUnits, kGroup = 32 / kU;  // steps whose units the lanes hold
+  const int blocks = (u1 - u0 + kU - 1) / kU;
+  const int steps = blocks > warp ? (blocks - warp + kWarps - 1) / kWarps : 0;
   const int32_t* table = a.tables + int64_t(b) * a.table_stride;
 
-  // Where the units of the next 16 steps are, two a step, one in every lane:
-  // byte offset in the pages and token in the page.  `have` has a bit for each.
+  // Where the units of the next kGroup steps are, one in every lane: byte
+  // offset in the pages and token in the page.  `have` has a bit for each.
   struct Units {
     int64_t offset;
     int within;
@@ -598,7 +649,7 @@ __device__ __forceinline__ void attend_segment(const AttnArgs& a, TileShared<D, 
   };
   auto fetch = [&](int step) {
     Units f{0, 0, 0u};
-    const int i = u0 + 2 * (warp + kWarps * (step + lane / 2)) + lane % 2;
+    const int i = u0 + kU * (warp + kWarps * (step + lane / kU)) + lane % kU;
     bool real = i < u1;
     if (real) {
       const int n = i < v.sink_units ? i : i + v.gap;
@@ -613,26 +664,24 @@ __device__ __forceinline__ void attend_segment(const AttnArgs& a, TileShared<D, 
     return f;
   };
   Units now = fetch(0), later{0, 0, 0u};
-  if (steps > 16) later = fetch(16);
-  uint32_t there = 0;  // which units of the steps in flight are there, two bits a step
+  if (steps > kGroup) later = fetch(kGroup);
+  uint32_t there = 0;  // which units of the steps in flight are there, kU bits a step
 
   // This lane's part of the copies: 16-byte pieces lane, lane + 32, ... of each
-  // unit's codes, and one piece of the four runs of scales and zeros.
+  // unit's codes, and one piece of the runs of scales and zeros.
   const int64_t head_at = int64_t(head) * a.cache.head_bytes;
   const uint8_t* key_from = a.cache.pages[0] + head_at + 16 * lane;
   const uint8_t* value_from = a.cache.pages[1] + head_at + 16 * lane;
-  const int param_unit = (lane / 4) % 2;
-  const uint8_t* param_from = a.cache.pages[(lane / 8) % 2] + head_at +
+  const int param_unit = (lane / 4) % kU;
+  const uint8_t* param_from = a.cache.pages[lane / (4 * kU) % 2] + head_at +
                               a.cache.block_size * (D / 2) + 16 * (lane % 4);
   auto load_step = [&](int step, uint32_t dst) {
-    const int at = 2 * (step % 16);
-    const uint32_t bits = (now.have >> at) & 3u;
-    there = (there << 2) | bits;
-    const int64_t offset[2] = {__shfl_sync(~0u, now.offset, at),
-                               __shfl_sync(~0u, now.offset, at + 1)};
-    const int within = __shfl_sync(~0u, now.within, at + param_unit);
+    const int at = kU * (step % kGroup);
+    const uint32_t bits = (now.have >> at) & ((1u << kU) - 1u);
+    there = (there << kU) | bits;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kU; ++u) {
+      const int64_t offset = __shfl_sync(~0u, now.offset, at + u);
       const int size = (bits >> u) & 1u ? 16 : 0;
 #pragma unroll
       for (int i = 0; i < S::kUnit / 512; ++i) {
@@ -642,20 +691,21 @@ __device__ __forceinline__ void attend_segment(const AttnArgs& a, TileShared<D, 
         const int vc = c ^ (D == 64    ? 2 * ((c >> 3) & 1)
                             : D == 128 ? 2 * ((c >> 3) & 3)
                                        : 2 * ((c >> 4) & 3));
-        copy16(dst + u * S::kUnit + 16 * kc, key_from + offset[u] + 512 * i, size);
-        copy16(dst + (2 + u) * S::kUnit + 16 * vc, value_from + offset[u] + 512 * i, size);
+        copy16(dst + u * S::kUnit + 16 * kc, key_from + offset + 512 * i, size);
+        copy16(dst + (kU + u) * S::kUnit + 16 * vc, value_from + offset + 512 * i, size);
       }
     }
-    if (lane < 16)
-      copy16(dst + 4 * S::kUnit + 16 * lane,
-             param_from + offset[param_unit] - within * (S::kUnit - 64),
+    const int64_t offset = __shfl_sync(~0u, now.offset, at + param_unit);
+    const int within = __shfl_sync(~0u, now.within, at + param_unit);
+    if (lane < 8 * kU)
+      copy16(dst + 2 * kU * S::kUnit + 16 * lane, param_from + offset - within * (S::kUnit - 64),
              (bits >> param_unit) & 1u ? 16 : 0);
   };
 
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
     if (i < steps) load_step(i, mine_s + i * S::kStage);
-    else there <<= 2;
+    else there <<= kU;
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   load_queries<T, D, NT>(a, s, row0, rows, head, sh);
@@ -678,7 +728,8 @@ __device__ __forceinline__ void attend_segment(const AttnArgs& a, TileShared<D, 
   st.c = 0.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    st.m[n] = make_float2(kNegInf, kNegInf), st.l[n] = make_float2(0.f, 0.f);
+    st.m[n] = make_float2(-kNegInf, -kNegInf), st.l[n] = make_float2(0.f, 0.f);
+    st.limit[n] = make_float2(kNegInf, kNegInf);
     st.z[n][0] = st.z[n][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -688,43 +739,34 @@ __device__ __forceinline__ void attend_segment(const AttnArgs& a, TileShared<D, 
     }
   }
 
-  // Pairs [plain_from, plain_from + plain_units) need no mask: behind no row,
-  // and inside every row's window.
+  // Steps that begin in [plain_from, plain_from + plain_units) need no mask:
+  // behind no row, and inside every row's window.
   const int plain_from = max(v.sink_units, (max(v.p_hi - a.window + 1, 0) + 15) / 16 - v.gap);
-  const unsigned plain_units = unsigned(max((v.p_lo + 1) / 16 - v.gap - plain_from - 1, 0));
+  const unsigned plain_units = unsigned(max((v.p_lo + 1) / 16 - v.gap - plain_from - (kU - 1), 0));
   const LaneAddress lane_at = lane_address<D>(mine_s, g, j);
   uint32_t buffer = 0, ahead = (kStages - 1) * S::kStage;  // bytes into the ring
-  int i = u0 + 2 * warp;
-  for (int step = 0; step < steps; ++step, i += 2 * kWarps) {
+  int i = u0 + kU * warp;
+  for (int step = 0; step < steps; ++step, i += kU * kWarps) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncwarp();
     const int next = step + kStages - 1;
-    if (next % 16 == 0) {
+    if (next % kGroup == 0) {
       now = later;
-      if (next + 16 < steps) later = fetch(next + 16);
+      if (next + kGroup < steps) later = fetch(next + kGroup);
     }
     if (next < steps) load_step(next, mine_s + ahead);
-    else there <<= 2;
+    else there <<= kU;
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const uint32_t bits = (there >> (2 * (kStages - 1))) & 3u;
-    const bool plain = bits == 3u && unsigned(i - plain_from) < plain_units;
+    const uint32_t bits = (there >> (kU * (kStages - 1))) & ((1u << kU) - 1u);
     const LaneAddress at = lane_at + buffer;
-    int number[2] = {0, 0};
-    if (!plain) {
-      number[0] = bits & 1u ? (i < v.sink_units ? i : i + v.gap) : -1;
-      number[1] = bits & 2u ? (i + 1 < v.sink_units ? i + 1 : i + 1 + v.gap) : -1;
-    }
-    if constexpr (NT <= 2) {
-      if (plain)
-        attend_units<D, NT, 0, 2, false>(a, sh, qreg, at, number, col, v, st);
-      else
-        attend_units<D, NT, 0, 2, true>(a, sh, qreg, at, number, col, v, st);
-    } else if (plain) {
-      attend_units<D, NT, 0, 1, false>(a, sh, qreg, at, number, col, v, st);
-      attend_units<D, NT, 1, 1, false>(a, sh, qreg, at, number, col, v, st);
+    if (bits == (1u << kU) - 1u && unsigned(i - plain_from) < plain_units) {
+      attend_step<D, NT, false>(a, sh, qreg, at, nullptr, col, v, st);
     } else {
-      attend_units<D, NT, 0, 1, true>(a, sh, qreg, at, number, col, v, st);
-      attend_units<D, NT, 1, 1, true>(a, sh, qreg, at, number, col, v, st);
+      int number[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        number[u] = (bits >> u) & 1u ? (i + u < v.sink_units ? i + u : i + u + v.gap) : -1;
+      attend_step<D, NT, true>(a, sh, qreg, at, number, col, v, st);
     }
     __syncwarp();
     buffer = buffer + S::kStage == S::kWarpBytes ? 0u : buffer + S::kStage;
@@ -744,7 +786,7 @@ __device__ __forceinline__ void attend_segment(const AttnArgs& a, TileShared<D, 
         st.z[n][c] += __shfl_xor_sync(~0u, st.z[n][c], d);
       }
       if (g == 0) {
-        sh.m[warp][8 * n + 2 * j + c] = c ? st.m[n].y : st.m[n].x;
+        sh.m[warp][8 * n + 2 * j + c] = c ? -st.m[n].y : -st.m[n].x;
         sh.l[warp][8 * n + 2 * j + c] = l;
       }
     }
@@ -851,7 +893,7 @@ __device__ __forceinline__ void item_of(const Work& w, int64_t in, int* item, in
 // share that begins or ends among an item's units leaves a partial result in
 // the workspace (at most two for a CTA), which q4_join brings together.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT <= 2 && D <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, 2)
     q4_attend(const __grid_constant__ AttnArgs a) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ TileShared<D, NT> sh;
