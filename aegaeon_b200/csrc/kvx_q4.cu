@@ -125,7 +125,9 @@ int tile_rows(int64_t rows, int64_t head_dim) {
 }
 
 // CTAs that are resident on the device at once.
-int resident(int sms) { return 2 * sms; }
+int resident(int rows, int64_t head_dim, int sms) {
+  return ctas_per_sm(int(head_dim), rows) * sms;
+}
 
 int sm_count(int* sms, int* device) {
   cudaError_t e = cudaGetDevice(device);
@@ -133,16 +135,18 @@ int sm_count(int* sms, int* device) {
   return e == cudaSuccess ? KVX_OK : cuda_fail("cudaDeviceGetAttribute", e);
 }
 
-// Items up to which the join takes a block for each row: a few dozen CTAs then
-// share an item, and the rows' blocks still fit the device at once.
-constexpr int64_t kJoinByRow = 64;
+// Items up to which the join takes a block for each row: 18 or more warps share
+// an item then, and the rows' blocks still fit the device in a wave or two.
+constexpr int64_t kJoinByItem = 64;
 
 uint64_t workspace_of(int rows, int64_t head_dim, int sms) {
-  return 2ull * resident(sms) * rows * (4 * head_dim + 8);
+  const uint64_t shares = uint64_t(kWarps) * resident(rows, head_dim, sms);
+  return 2 * shares * rows * (4 * head_dim + 8) + shares * sizeof(Joint);
 }
 
 template <typename T, int D, int NT>
-int launch_attention(const AttnArgs& a, int grid, int64_t items, int device, cudaStream_t s) {
+int launch_attention(const AttnArgs& a, int grid, int64_t items, double bound,
+                     int device, cudaStream_t s) {
   constexpr int shared = Shape<D>::kShared;
   static std::atomic<uint64_t> allowed{0};  // devices that know the shared-memory size
   cudaError_t e = cudaSuccess;
@@ -156,40 +160,39 @@ int launch_attention(const AttnArgs& a, int grid, int64_t items, int device, cud
   q4_attend<T, D, NT><<<grid, kThreads, shared, s>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail("q4_attend", e);
-  if (grid == 1) return KVX_OK;  // one CTA has the whole of every item
-  // The join's launch and its search for its item overlap the attention.
-  // A block for each row where there are fewer items than a warp would have
-  // pieces to walk through, otherwise one for each border between shares.
-  const bool by_row = items <= kJoinByRow;
+  if (bound <= 1) return KVX_OK;  // one share has the whole of every item
+  // The join's launch overlaps the attention.
+  const int shares = grid * kWarps;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(by_row ? unsigned(items * 8 * NT) : unsigned(grid - 1));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(unsigned(a.joint_by_item ? items * 8 * NT
+                                              : (shares + kJoinWarps - 1) / kJoinWarps));
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = by_row ? cudaLaunchKernelEx(&cfg, q4_join<T, D, NT, true>, a, grid)
-             : cudaLaunchKernelEx(&cfg, q4_join<T, D, NT, false>, a, grid);
+  e = a.joint_by_item ? cudaLaunchKernelEx(&cfg, q4_join<T, D, NT, true>, a, shares)
+                      : cudaLaunchKernelEx(&cfg, q4_join<T, D, NT, false>, a, shares);
   return e == cudaSuccess ? KVX_OK : cuda_fail("q4_join", e);
 }
 
 template <typename T>
 int launch_attention(const AttnArgs& a, int64_t head_dim, int rows, int grid, int64_t items,
-                     int device, cudaStream_t s) {
+                     double bound, int device, cudaStream_t s) {
   if (head_dim == 64) {
-    if (rows == 8) return launch_attention<T, 64, 1>(a, grid, items, device, s);
-    if (rows == 16) return launch_attention<T, 64, 2>(a, grid, items, device, s);
-    return launch_attention<T, 64, 4>(a, grid, items, device, s);
+    if (rows == 8) return launch_attention<T, 64, 1>(a, grid, items, bound, device, s);
+    if (rows == 16) return launch_attention<T, 64, 2>(a, grid, items, bound, device, s);
+    return launch_attention<T, 64, 4>(a, grid, items, bound, device, s);
   }
   if (head_dim == 128) {
-    if (rows == 8) return launch_attention<T, 128, 1>(a, grid, items, device, s);
-    if (rows == 16) return launch_attention<T, 128, 2>(a, grid, items, device, s);
-    return launch_attention<T, 128, 4>(a, grid, items, device, s);
+    if (rows == 8) return launch_attention<T, 128, 1>(a, grid, items, bound, device, s);
+    if (rows == 16) return launch_attention<T, 128, 2>(a, grid, items, bound, device, s);
+    return launch_attention<T, 128, 4>(a, grid, items, bound, device, s);
   }
-  if (rows == 8) return launch_attention<T, 256, 1>(a, grid, items, device, s);
-  return launch_attention<T, 256, 2>(a, grid, items, device, s);
+  if (rows == 8) return launch_attention<T, 256, 1>(a, grid, items, bound, device, s);
+  return launch_attention<T, 256, 2>(a, grid, items, bound, device, s);
 }
 
 }  // namespace
@@ -325,22 +328,23 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   a.upp_shift = -1;
   for (int i = 0; i < 9; ++i)
     if (a.upp == 1 << i) a.upp_shift = i;
-  // Shares: the CTAs that are resident at once, or fewer where even the longest
-  // sequences that the tables can hold give them less than kMinUnits each.
+  // CTAs: those that are resident at once, or fewer where even the longest
+  // sequences that the tables can hold have too few units for their warps.
   const int64_t tiles = query_starts ? num_tokens * group / rows + batch
                                      : batch * ((queries * group + rows - 1) / rows);
   const int64_t units = std::max<int64_t>(table_width * a.upp, 1);
-  int64_t grid = resident(sms);
   const int64_t items = tiles * kv_heads;
-  const double bound =
-      double(items) * double(units + kItemUnits) / double(kMinUnits + kItemUnits);
-  if (bound < double(grid)) grid = std::max<int64_t>(1, int64_t(std::ceil(bound)));
-  const int64_t pieces = 2ll * resident(sms) * rows;
+  int64_t grid = resident(rows, head_dim, sms);
+  const double bound = double(items) * double(units);
+  if (bound < double(grid * kWarps)) grid = (int64_t(bound) + kWarps - 1) / kWarps;
+  const int64_t pieces = 2ll * kWarps * resident(rows, head_dim, sms) * rows;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * head_dim);
+  a.joints = reinterpret_cast<Joint*>(a.part_ml + pieces);
+  a.joint_by_item = !query_starts && items <= kJoinByItem;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == kBf16 ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), items, device, s)
-                        : launch_attention<__half>(a, head_dim, rows, int(grid), items, device, s);
+  return dtype == kBf16 ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), items, bound, device, s)
+                        : launch_attention<__half>(a, head_dim, rows, int(grid), items, bound, device, s);
 }
 
 }  // extern "C"

@@ -21,13 +21,23 @@ namespace q4 {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 3;       // steps in flight or in use, per warp
+constexpr int kStages = 2;       // a step in use and one in flight, per warp
+constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr int kNoWindow = 1 << 30;
-// Fewest 16-token units a CTA takes: four for each warp, a whole step.
-constexpr int kMinUnits = 4 * kWarps;
-// What an item (a tile of query rows with one kv head) costs besides its units,
-// in units: its queries, its first block ids and the join of the warps.
-constexpr int kItemUnits = 16;
+// What an item (a tile of query rows with one kv head) costs a warp besides its
+// 16-token units, in units: its queries, its first block ids, its result.
+constexpr int kItemUnits = 3;
+// Fewest units of a share when items are cut wherever shares end.
+constexpr int kMinShare = 8;
+// Sizes of the pieces that items may be cut into instead: 1 << 0 ... kPieces - 1.
+constexpr int kPieces = 6;
+// CTAs that an SM holds.
+__host__ __device__ constexpr int ctas_per_sm(int head_dim, int rows) {
+  return head_dim == 256 && rows > 8 ? 1 : 2;
+}
+
+struct Joint;
 
 struct AttnArgs {
   Cache cache;
@@ -52,8 +62,10 @@ struct AttnArgs {
   int upp;                  // 16-token units of a page
   int upp_shift;            // log2(upp), -1 when it is no power of two
   int q_vec, o_vec;         // 16-byte accesses serve for query / out
-  float* part_o;            // [2 * grid][rows][D]
-  float2* part_ml;          // [2 * grid][rows] (running maximum, sum)
+  float* part_o;            // [2 * shares][rows][D]
+  float2* part_ml;          // [2 * shares][rows] (running maximum, sum)
+  Joint* joints;            // [shares], or [items]
+  int joint_by_item;
 };
 
 struct Seq {
@@ -99,49 +111,6 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Seq& s, int row
   return v;
 }
 
-// Work of all sequences, and the place of a position in its running sum.  Every
-// thread takes a run of sequences; `at` maps the total to the position.
-struct Place {
-  int index;       // the sequence whose part holds the position, n when none does
-  int64_t before;  // work of the sequences before it
-};
-
-template <class F, class G>
-__device__ __forceinline__ int64_t block_locate(F f, int n, G at, int64_t* sm, Place* found,
-                                                Place* place) {
-  const int run = (n + kThreads - 1) / kThreads, first = threadIdx.x * run;
-  const int last = min(first + run, n);
-  int64_t own = 0;
-  for (int i = first; i < last; ++i) own += f(i);
-  int64_t v = own;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const int64_t u = __shfl_up_sync(~0u, v, d);
-    if (threadIdx.x % 32 >= d) v += u;
-  }
-  if (threadIdx.x % 32 == 31) sm[threadIdx.x / 32] = v;
-  if (threadIdx.x == 0) *found = Place{n, 0};
-  __syncthreads();
-  int64_t before = v - own, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < int(threadIdx.x / 32)) before += sm[w];
-    total += sm[w];
-  }
-  const int64_t pos = at(total);
-  if (pos >= before && pos < before + own) {
-    int i = first;
-    for (int64_t c = run > 1 ? f(i) : own; pos >= before + c; c = f(i)) {
-      before += c;
-      ++i;
-    }
-    *found = Place{i, before};
-  }
-  __syncthreads();
-  *place = *found;
-  return total;
-}
-
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -181,9 +150,7 @@ struct Shape {
   static constexpr int kParams = kUnits * 64;   // (scale, zero) of the units' tokens, one tensor
   static constexpr int kStage = kUnits * 2 * kUnit + 2 * kParams;
   static constexpr int kWarpBytes = kStages * kStage;
-  static constexpr int kRing = kWarps * kWarpBytes;
-  static constexpr int kJoin = kWarps * 8 * (D + 4) * 4;
-  static constexpr int kShared = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kShared = kWarps * kWarpBytes;
   static constexpr int kKeyWords = D / 32;      // code words of a thread for one token of K
 };
 
@@ -194,86 +161,98 @@ __device__ __forceinline__ int key_dim(int j, int w) {
   return D == 256 ? (w / 4) * 128 + 32 * j + 8 * (w % 4) : (D / 4) * j + 8 * w;
 }
 
-// Rows of one tile of queries as the CTA keeps them.
-template <int D, int NT>
-struct TileShared {
-  uint2 q[NT][D / 16][32];  // B fragments of the queries, as mma reads them
-  float factor[NT * 8];     // |scale| * log2(e) and the powers of two taken out
-  float sum[NT * 8];        // sum(q) in the unit of the products with the codes
-  int pos[NT * 8];          // position in the sequence, -1 for rows that are none
-  float m[kWarps][NT * 8];
-  float l[kWarps][NT * 8];
-  int64_t scan[kWarps];
-  Place place;
+// What a thread keeps of the tile's rows (its columns 2j, 2j + 1 of each eight).
+template <int NT>
+struct Columns {
+  float2 factor[NT];  // on the raw score: |scale| * log2(e) and the powers of two taken out
+  float2 sum[NT];     // sum(q), in the raw score's unit
+  int pos[NT][2];     // position in the sequence, -1 for rows that are none
 };
 
-// Query rows of a tile into B fragments.  A row is scaled by a power of two so
-// that its largest element lies in [2^14, 2^15): every 16-bit float within
-// 2^-28 of it stays exact in fp16, whatever the row's range.
+// B fragments of the queries, as mma reads them: in registers for a tile of
+// eight rows, otherwise in the warp's shared memory.
+template <int D, int NT>
+struct Fragments {
+  uint2 reg[NT == 1 ? D / 16 : 1];
+  uint2* shared;  // [NT][D / 16][32], this lane's
+  __device__ __forceinline__ uint2 at(int n, int k) const {
+    return NT == 1 ? reg[k] : shared[(n * (D / 16) + k) * 32];
+  }
+  __device__ __forceinline__ void set(int n, int k, uint2 x) {
+    if constexpr (NT == 1) reg[k] = x;
+    else shared[(n * (D / 16) + k) * 32] = x;
+  }
+};
+
+// A tile's query rows.  A row is scaled by a power of two so that its largest
+// element lies in [2^14, 2^15): every 16-bit float within 2^-28 of it stays
+// exact in fp16, whatever the row's range.
 template <typename T, int D, int NT>
 __device__ __forceinline__ void load_queries(const AttnArgs& a, const Seq& s, int row0, int rows,
-                                             int head, TileShared<D, NT>& sh) {
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
-  static_assert(NT <= kWarps, "a warp for each eight rows");
-  if (warp >= NT) return;
-  const int r = warp * 8 + g;
-  const bool real = r < rows;
-  constexpr int kW = Shape<D>::kKeyWords;
-  float x[kW][8];
-  const T* base = static_cast<const T*>(a.query);
-  int pos = -1;
-  if (real) {
-    const int token = (row0 + r) / a.group, h = (row0 + r) % a.group;
-    pos = s.len - s.count + token;
-    base += int64_t(s.start + token) * a.q_token + int64_t(head * a.group + h) * a.q_head;
-  }
-  float top = 0.f, sum = 0.f;
+                                             int head, Fragments<D, NT>& f, Columns<NT>& col) {
+  const int lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
+  constexpr int kW = D / 32;
 #pragma unroll
-  for (int w = 0; w < kW; ++w) {
-    const T* p = base + key_dim<D>(j, w);
-    T v[8];
-    if (!real) {
+  for (int n = 0; n < NT; ++n) {
+    const int r = 8 * n + g;
+    const bool real = r < rows;
+    float x[kW][8];
+    const T* base = static_cast<const T*>(a.query);
+    int pos = -1;
+    if (real) {
+      const int token = (row0 + r) / a.group, h = (row0 + r) - token * a.group;
+      pos = s.len - s.count + token;
+      base += int64_t(s.start + token) * a.q_token + int64_t(head * a.group + h) * a.q_head;
+    }
+    float top = 0.f, sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = from_float<T>(0.f);
-    } else if (a.q_vec) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      __builtin_memcpy(v, &u, 16);
-    } else {
+    for (int w = 0; w < kW; ++w) {
+      const T* p = base + key_dim<D>(j, w);
+      T v[8];
+      if (!real) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = p[i];
+        for (int i = 0; i < 8; ++i) v[i] = from_float<T>(0.f);
+      } else if (a.q_vec) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        __builtin_memcpy(v, &u, 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[w][i] = to_float(v[i]);
+        top = fmaxf(top, fabsf(x[w][i]));
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[w][i] = to_float(v[i]);
-      top = fmaxf(top, fabsf(x[w][i]));
+    for (int d = 1; d < 4; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    // 2^(14 - exponent of top); bounded so that both it and its inverse are normal.
+    const int e = min(max(int(__float_as_uint(top) >> 23), 20), 250);
+    float up = top > 0.f ? __uint_as_float(uint32_t(min(127 + 14 + 127 - e, 240)) << 23) : 1.f;
+    const float factor = fmaxf(a.scale_log2 * 16777216.f / up, 1e-37f);  // never 0: hidden
+    up *= a.sign;                                                        // scores are -inf
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      uint32_t b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float u = (i % 2) ? up * 0.0625f : up;  // odd nibbles are 16 times as large
+        const __half2 h = __floats2half2_rn(x[w][i] * u, x[w][i + 4] * u);
+        sum += x[w][i] * up + x[w][i + 4] * up;
+        __builtin_memcpy(&b[i], &h, 4);
+      }
+      f.set(n, 2 * w, make_uint2(b[0], b[1]));
+      f.set(n, 2 * w + 1, make_uint2(b[2], b[3]));
     }
-  }
 #pragma unroll
-  for (int d = 1; d < 4; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-  // 2^(14 - exponent of top); bounded so that both it and its inverse are normal.
-  const int e = min(max(int(__float_as_uint(top) >> 23), 20), 250);
-  float up = top > 0.f ? __uint_as_float(uint32_t(min(127 + 14 + 127 - e, 240)) << 23) : 1.f;
-  const float factor = a.scale_log2 * 16777216.f / up;
-  up *= a.sign;
-#pragma unroll
-  for (int w = 0; w < kW; ++w) {
-    uint32_t f[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float u = (i % 2) ? up * 0.0625f : up;  // odd nibbles are 16 times as large
-      const __half2 h = __floats2half2_rn(x[w][i] * u, x[w][i + 4] * u);
-      sum += x[w][i] * up + x[w][i + 4] * up;
-      __builtin_memcpy(&f[i], &h, 4);
-    }
-    sh.q[warp][2 * w][lane] = make_uint2(f[0], f[1]);
-    sh.q[warp][2 * w + 1][lane] = make_uint2(f[2], f[3]);
-  }
-#pragma unroll
-  for (int d = 1; d < 4; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
-  if (j == 0) {
-    sh.factor[r] = fmaxf(factor, 1e-37f);  // never 0: hidden scores are -inf
-    sh.sum[r] = sum * 5.9604644775390625e-8f;
-    sh.pos[r] = pos;
+    for (int d = 1; d < 4; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
+    sum *= 5.9604644775390625e-8f;
+    // Row 2j is with the lanes 8j ..., row 2j + 1 four lanes on.
+    col.factor[n] = make_float2(__shfl_sync(~0u, factor, 8 * j), __shfl_sync(~0u, factor, 8 * j + 4));
+    col.sum[n] = make_float2(__shfl_sync(~0u, sum, 8 * j), __shfl_sync(~0u, sum, 8 * j + 4));
+    col.pos[n][0] = __shfl_sync(~0u, pos, 8 * j);
+    col.pos[n][1] = __shfl_sync(~0u, pos, 8 * j + 4);
   }
 }
 
@@ -372,8 +351,8 @@ __device__ __forceinline__ void value_words(uint32_t a, uint32_t (&w)[D / 64]) {
 
 // q . c of one unit's 16 tokens with the tile's rows.
 template <int D, int NT, int U>
-__device__ __forceinline__ void unit_scores(const LaneAddress& at, const TileShared<D, NT>& sh,
-                                            const uint2* qreg, float (&x)[NT][4]) {
+__device__ __forceinline__ void unit_scores(const LaneAddress& at, const Fragments<D, NT>& f,
+                                            float (&x)[NT][4]) {
   constexpr int kW = D / 32;
   uint32_t lo[kW], hi[kW];
   key_words<D, U, 0>(at, lo);
@@ -389,7 +368,7 @@ __device__ __forceinline__ void unit_scores(const LaneAddress& at, const TileSha
       const uint32_t r0 = h ? lo[w] >> 8 : lo[w], r1 = h ? hi[w] >> 8 : hi[w];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const uint2 q = NT == 1 ? qreg[2 * w + h] : sh.q[n][2 * w + h][threadIdx.x % 32];
+        const uint2 q = f.at(n, 2 * w + h);
         mma(x[n], r0 & kEven, r1 & kEven, r0 & kOdd, r1 & kOdd, q.x, q.y);
       }
     }
@@ -422,14 +401,6 @@ __device__ __forceinline__ void unit_values(const LaneAddress& at, const uint32_
     mma(st.ps[n], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, b[n][0], b[n][1]);
 }
 
-// What a thread keeps of the tile's rows (its columns 2j, 2j + 1 of each eight).
-template <int NT>
-struct Columns {
-  float2 factor[NT];  // on the raw score: scale * log2(e) and the powers of two
-  float2 sum[NT];     // sum(q), in the raw score's unit
-  int pos[NT][2];
-};
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -452,8 +423,8 @@ __device__ __forceinline__ void each(F f) {
 // kAb units from unit U of the stage on: scores, softmax, products.  `number`
 // gives the units' numbers in the sequence, -1 for one that is not there.
 template <int D, int NT, int U, int kAb, bool kMasked>
-__device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared<D, NT>& sh,
-                                             const uint2* qreg, const LaneAddress& at,
+__device__ __forceinline__ void attend_units(const AttnArgs& a, const Fragments<D, NT>& f,
+                                             const LaneAddress& at,
                                              const int* number, const Columns<NT>& col,
                                              const Span& v, WarpState<D, NT>& st) {
   const int lane = threadIdx.x % 32, g = lane / 4;
@@ -465,7 +436,7 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
     kp[u][0] = lds32<at_u>(at.p), kp[u][1] = lds32<at_u + 32>(at.p);
     vp[u][0] = lds32<Shape<D>::kParams + at_u>(at.p);
     vp[u][1] = lds32<Shape<D>::kParams + at_u + 32>(at.p);
-    unit_scores<D, NT, U + u>(at, sh, qreg, x[u]);
+    unit_scores<D, NT, U + u>(at, f, x[u]);
   });
   float vs[kAb][2], vz[kAb][2], most = 0.f;
 #pragma unroll
@@ -522,7 +493,7 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float f[2];
+      float by[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float factor = c ? col.factor[n].y : col.factor[n].x;
@@ -530,17 +501,17 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
         float t = fmaxf(top[n][c] * factor, -m);
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
-        f[c] = t == kNegInf ? 1.f : ex2(-m - t);
+        by[c] = t == kNegInf ? 1.f : ex2(-m - t);
         m = -t;
         (c ? st.limit[n].y : st.limit[n].x) = (t + 8.f) / factor;
       }
-      st.l[n].x *= f[0], st.l[n].y *= f[1];
-      st.z[n][0] *= f[0], st.z[n][1] *= f[1];
+      st.l[n].x *= by[0], st.l[n].y *= by[1];
+      st.z[n][0] *= by[0], st.z[n][1] *= by[1];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        st.ps[n][i] *= f[i % 2] * ratio;
+        st.ps[n][i] *= by[i % 2] * ratio;
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) st.o[n][d][i] *= f[i % 2] * ratio;
+        for (int d = 0; d < D / 16; ++d) st.o[n][d][i] *= by[i % 2] * ratio;
       }
     }
   }
@@ -579,23 +550,36 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const TileShared
   });
 }
 
-// The units of a step, as many at a time as the registers hold.
-template <int D, int NT, bool kMasked>
-__device__ __forceinline__ void attend_step(const AttnArgs& a, const TileShared<D, NT>& sh,
-                                            const uint2* qreg, const LaneAddress& at,
-                                            const int* number, const Columns<NT>& col,
-                                            const Span& v, WarpState<D, NT>& st) {
-  constexpr int kAll = Shape<D>::kUnits;
-  constexpr int kAb = NT == 4 ? 1 : NT == 2 || D == 256 || kMasked ? 2 : 4;
-  each<kAll / kAb>([&](auto index) {
-    constexpr int kFirst = decltype(index)::value * kAb;
-    if constexpr (kMasked) {  // units behind the last are not there
-      bool any = false;
-#pragma unroll
-      for (int u = 0; u < kAb; ++u) any |= number[kFirst + u] >= 0;
-      if (!any) return;
+// The units of a step.  `plain`: bits of those that need no mask; `there`: of those that
+// are there at all; the first is number i of the tile's units.
+template <int D, int NT>
+__device__ __forceinline__ void attend_step(const AttnArgs& a, const Fragments<D, NT>& f,
+                                            const LaneAddress& at, uint32_t there, uint32_t plain,
+                                            int i, const Columns<NT>& col, const Span& v,
+                                            WarpState<D, NT>& st) {
+  constexpr int kU = Shape<D>::kUnits;
+  constexpr uint32_t kAll = (1u << kU) - 1u;
+  if constexpr (NT == 1 && kU == 4) {
+    if (plain == kAll) {
+      attend_units<D, NT, 0, 4, false>(a, f, at, nullptr, col, v, st);
+      return;
     }
-    attend_units<D, NT, kFirst, kAb, kMasked>(a, sh, qreg, at, number + kFirst, col, v, st);
+  }
+  constexpr int kAb = NT == 4 ? 1 : 2;  // as many at a time as the registers hold
+  constexpr uint32_t kPart = (1u << kAb) - 1u;
+  each<kU / kAb>([&](auto index) {
+    constexpr int kFirst = decltype(index)::value * kAb;
+    if (((plain >> kFirst) & kPart) == kPart) {
+      attend_units<D, NT, kFirst, kAb, false>(a, f, at, nullptr, col, v, st);
+    } else if ((there >> kFirst) & kPart) {
+      int number[kAb];
+#pragma unroll
+      for (int u = 0; u < kAb; ++u) {
+        const int k = i + kFirst + u;
+        number[u] = (there >> (kFirst + u)) & 1u ? (k < v.sink_units ? k : k + v.gap) : -1;
+      }
+      attend_units<D, NT, kFirst, kAb, true>(a, f, at, number, col, v, st);
+    }
   });
 }
 
@@ -623,242 +607,42 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const Seq& s, int r
         l == 0.f ? kNegInf : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// The units [u0, u1) of one (tile of query rows, kv head): every warp takes
-// pairs of units in turn through its own ring of cp.async stages, then the
-// warps' results are joined.  `slot` < 0: the result is the tile's output,
-// otherwise it goes to that place of the workspace.
-template <typename T, int D, int NT>
-__device__ __forceinline__ void attend_segment(const AttnArgs& a, TileShared<D, NT>& sh, uint8_t* ring, int b,
-                               const Seq& s, const Span& v, int row0, int rows, int head, int u0,
-                               int u1, int slot) {
-  using S = Shape<D>;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
-  uint8_t* mine = ring + warp * S::kWarpBytes;
-  const uint32_t mine_s = uint32_t(__cvta_generic_to_shared(mine));
-  constexpr int kU = S::kUnits, kGroup = 32 / kU;  // steps whose units the lanes hold
-  const int blocks = (u1 - u0 + kU - 1) / kU;
-  const int steps = blocks > warp ? (blocks - warp + kWarps - 1) / kWarps : 0;
-  const int32_t* table = a.tables + int64_t(b) * a.table_stride;
-
-  // Where the units of the next kGroup steps are, one in every lane: byte
-  // offset in the pages and token in the page.  `have` has a bit for each.
-  struct Units {
-    int64_t offset;
-    int within;
-    uint32_t have;
-  };
-  auto fetch = [&](int step) {
-    Units f{0, 0, 0u};
-    const int i = u0 + kU * (warp + kWarps * (step + lane / kU)) + lane % kU;
-    bool real = i < u1;
-    if (real) {
-      const int n = i < v.sink_units ? i : i + v.gap;
-      const int page = a.upp_shift >= 0 ? n >> a.upp_shift : n / a.upp;
-      const int id = table[page];
-      f.within = n - page * a.upp;
-      real = id >= 0 && id < a.cache.num_blocks;
-      if (real) f.offset = id * a.cache.stride + f.within * S::kUnit;
-      else atomicExch(&g_q4_status, 5 /* KVX_ERR_BLOCK_ID */);
-    }
-    f.have = __ballot_sync(~0u, real);
-    return f;
-  };
-  Units now = fetch(0), later{0, 0, 0u};
-  if (steps > kGroup) later = fetch(kGroup);
-  uint32_t there = 0;  // which units of the steps in flight are there, kU bits a step
-
-  // This lane's part of the copies: 16-byte pieces lane, lane + 32, ... of each
-  // unit's codes, and one piece of the runs of scales and zeros.
-  const int64_t head_at = int64_t(head) * a.cache.head_bytes;
-  const uint8_t* key_from = a.cache.pages[0] + head_at + 16 * lane;
-  const uint8_t* value_from = a.cache.pages[1] + head_at + 16 * lane;
-  const int param_unit = (lane / 4) % kU;
-  const uint8_t* param_from = a.cache.pages[lane / (4 * kU) % 2] + head_at +
-                              a.cache.block_size * (D / 2) + 16 * (lane % 4);
-  auto load_step = [&](int step, uint32_t dst) {
-    const int at = kU * (step % kGroup);
-    const uint32_t bits = (now.have >> at) & ((1u << kU) - 1u);
-    there = (there << kU) | bits;
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int64_t offset = __shfl_sync(~0u, now.offset, at + u);
-      const int size = (bits >> u) & 1u ? 16 : 0;
-#pragma unroll
-      for (int i = 0; i < S::kUnit / 512; ++i) {
-        // The pieces' places are permuted so that the fragments' reads meet no bank twice.
-        const int c = lane + 32 * i;
-        const int kc = D == 256 ? c ^ (4 * ((c >> 3) & 1)) : c;
-        const int vc = c ^ (D == 64    ? 2 * ((c >> 3) & 1)
-                            : D == 128 ? 2 * ((c >> 3) & 3)
-                                       : 2 * ((c >> 4) & 3));
-        copy16(dst + u * S::kUnit + 16 * kc, key_from + offset + 512 * i, size);
-        copy16(dst + (kU + u) * S::kUnit + 16 * vc, value_from + offset + 512 * i, size);
-      }
-    }
-    const int64_t offset = __shfl_sync(~0u, now.offset, at + param_unit);
-    const int within = __shfl_sync(~0u, now.within, at + param_unit);
-    if (lane < 8 * kU)
-      copy16(dst + 2 * kU * S::kUnit + 16 * lane, param_from + offset - within * (S::kUnit - 64),
-             (bits >> param_unit) & 1u ? 16 : 0);
-  };
-
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (i < steps) load_step(i, mine_s + i * S::kStage);
-    else there <<= kU;
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-  load_queries<T, D, NT>(a, s, row0, rows, head, sh);
-  __syncthreads();
-
-  Columns<NT> col;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int c = 8 * n + 2 * j;
-    col.factor[n] = make_float2(sh.factor[c], sh.factor[c + 1]);
-    col.sum[n] = make_float2(sh.sum[c], sh.sum[c + 1]);
-    col.pos[n][0] = sh.pos[c], col.pos[n][1] = sh.pos[c + 1];
-  }
-  uint2 qreg[NT == 1 ? D / 16 : 1];
-  if constexpr (NT == 1) {
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) qreg[i] = sh.q[0][i][lane];
-  }
-  WarpState<D, NT> st;
-  st.c = 0.f;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    st.m[n] = make_float2(-kNegInf, -kNegInf), st.l[n] = make_float2(0.f, 0.f);
-    st.limit[n] = make_float2(kNegInf, kNegInf);
-    st.z[n][0] = st.z[n][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      st.ps[n][i] = 0.f;
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) st.o[n][d][i] = 0.f;
-    }
-  }
-
-  // Steps that begin in [plain_from, plain_from + plain_units) need no mask:
-  // behind no row, and inside every row's window.
-  const int plain_from = max(v.sink_units, (max(v.p_hi - a.window + 1, 0) + 15) / 16 - v.gap);
-  const unsigned plain_units = unsigned(max((v.p_lo + 1) / 16 - v.gap - plain_from - (kU - 1), 0));
-  const LaneAddress lane_at = lane_address<D>(mine_s, g, j);
-  uint32_t buffer = 0, ahead = (kStages - 1) * S::kStage;  // bytes into the ring
-  int i = u0 + kU * warp;
-  for (int step = 0; step < steps; ++step, i += kU * kWarps) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    __syncwarp();
-    const int next = step + kStages - 1;
-    if (next % kGroup == 0) {
-      now = later;
-      if (next + kGroup < steps) later = fetch(next + kGroup);
-    }
-    if (next < steps) load_step(next, mine_s + ahead);
-    else there <<= kU;
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    const uint32_t bits = (there >> (kU * (kStages - 1))) & ((1u << kU) - 1u);
-    const LaneAddress at = lane_at + buffer;
-    if (bits == (1u << kU) - 1u && unsigned(i - plain_from) < plain_units) {
-      attend_step<D, NT, false>(a, sh, qreg, at, nullptr, col, v, st);
-    } else {
-      int number[kU];
-#pragma unroll
-      for (int u = 0; u < kU; ++u)
-        number[u] = (bits >> u) & 1u ? (i + u < v.sink_units ? i + u : i + u + v.gap) : -1;
-      attend_step<D, NT, true>(a, sh, qreg, at, number, col, v, st);
-    }
-    __syncwarp();
-    buffer = buffer + S::kStage == S::kWarpBytes ? 0u : buffer + S::kStage;
-    ahead = ahead + S::kStage == S::kWarpBytes ? 0u : ahead + S::kStage;
-  }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-
-  // Join the warps.  Sums over the tokens of a thread's rows first.
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float l = c ? st.l[n].y : st.l[n].x;
-#pragma unroll
-      for (int d = 4; d < 32; d *= 2) {
-        l += __shfl_xor_sync(~0u, l, d);
-        st.z[n][c] += __shfl_xor_sync(~0u, st.z[n][c], d);
-      }
-      if (g == 0) {
-        sh.m[warp][8 * n + 2 * j + c] = c ? -st.m[n].y : -st.m[n].x;
-        sh.l[warp][8 * n + 2 * j + c] = l;
-      }
-    }
-  const float back = st.c > 0.f ? 1.f / st.c : 0.f;
-  float* join = reinterpret_cast<float*>(ring);
-  constexpr int kPitch = D + 4;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    if (8 * n >= rows) break;  // the same for the whole block
-    __syncthreads();           // the ring, or the previous rows, are read
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float* to = join + (warp * 8 + 2 * j + c) * kPitch + g * (D / 8);
-      const float mid = 7.5f * st.ps[n][c];
-#pragma unroll
-      for (int d = 0; d < D / 16; d += 2) {
-        float4 f;
-        f.x = fmaf(fmaf(st.o[n][d][c], 16777216.f, -mid), back, st.z[n][c]);
-        f.y = fmaf(fmaf(st.o[n][d][2 + c], 1048576.f, -mid), back, st.z[n][c]);
-        f.z = fmaf(fmaf(st.o[n][d + 1][c], 16777216.f, -mid), back, st.z[n][c]);
-        f.w = fmaf(fmaf(st.o[n][d + 1][2 + c], 1048576.f, -mid), back, st.z[n][c]);
-        *reinterpret_cast<float4*>(to + 2 * d) = f;
-      }
-    }
-    __syncthreads();
-    for (int e = threadIdx.x * 4; e < 8 * D; e += kThreads * 4) {
-      const int r = 8 * n + e / D, d = e % D;
-      if (r >= rows) continue;
-      float m = kNegInf;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.m[w][r]);
-      float l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float mw = sh.m[w][r], lw = sh.l[w][r];
-        // A warp without a finite score counts for nothing, unless a NaN is among them.
-        const float f = mw == kNegInf ? (lw == lw ? 0.f : lw) : ex2(mw - m);
-        if (f != 0.f) {
-          const float4 x = *reinterpret_cast<const float4*>(join + (w * 8 + r % 8) * kPitch + d);
-          l = fmaf(f, lw, l);
-          o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y);
-          o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
-        }
-      }
-      if (slot >= 0) {
-        *reinterpret_cast<float4*>(a.part_o + (int64_t(slot) * (8 * NT) + r) * D + d) = o;
-        if (d == 0) a.part_ml[int64_t(slot) * (8 * NT) + r] = make_float2(m, l);
-      } else {
-        store_row<T>(a, s, row0 + r, head, d, o, m, l);
-      }
-    }
-  }
-  __syncthreads();  // before the ring and the rows are used again
-}
-
 // Rows of a tile that see nothing.
 template <typename T, int D>
 __device__ __forceinline__ void store_nothing(const AttnArgs& a, const Seq& s, int row0, int rows,
                                               int head) {
-  for (int e = threadIdx.x; e < rows * (D / 4); e += kThreads)
+  for (int e = threadIdx.x % 32; e < rows * (D / 4); e += 32)
     store_row<T>(a, s, row0 + e / (D / 4), head, e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f),
                  kNegInf, 0.f);
 }
 
-// What a sequence adds to the work: items of one tile of query rows with one kv
-// head, each counted as long as the longest of the sequence's tiles, behind
-// kItemUnits for what an item costs besides.
-struct Work {
+// ---- how the work is shared --------------------------------------------------
+// An item is one tile of query rows with one kv head; it is counted as long as
+// the longest of its sequence's tiles.  The warps of a grid that is resident at
+// once take equal shares of all items, in one of two ways:
+//   pieces: every item is cut into pieces of `piece` units and a share is a
+//     piece: where that leaves no more pieces than warps, which have little each;
+//   running: an item counts units + kItemUnits, and shares end wherever they do.
+// A warp works alone: no barrier, and short items cost it little.  (With a CTA's
+// four warps on one item and their results joined in shared memory, 16 requests
+// of 1024 to 2048 tokens with 32 kv heads took 42 us.)  What a call's sequences are
+// is known on the device only, so every CTA works the plan out from the lengths.
+struct Plan {
+  int piece;      // 0: running
+  int64_t share;  // length of a share (pieces: 1)
+  __device__ __forceinline__ int length(int units) const {  // of an item
+    return piece ? max((units + piece - 1) / piece, 1) : units + kItemUnits;
+  }
+  // Unit at which a position of an item begins.
+  __device__ __forceinline__ int unit(int units, int off) const {
+    return piece ? min(off * piece, units) : max(off - kItemUnits, 0);
+  }
+};
+
+struct Work {  // of one sequence
   Seq s;
   int rows, tiles, units;
-  int64_t total;
+  int64_t items;
 };
 
 template <int ROWS>
@@ -868,229 +652,538 @@ __device__ __forceinline__ Work work_of(const AttnArgs& a, int b) {
   w.rows = w.s.count * a.group;
   w.tiles = (w.rows + ROWS - 1) / ROWS;
   w.units = span_of(a, w.s, 0, w.rows).units;
-  w.total = int64_t(w.units + kItemUnits) * w.tiles * a.cache.kv_heads;
+  w.items = int64_t(w.tiles) * a.cache.kv_heads;
   return w;
 }
 
-__device__ __forceinline__ int64_t share_of(int64_t total, int shares) {
-  return max(int64_t(kMinUnits + kItemUnits), (total + shares - 1) / shares);
-}
+// The plan, and the place of the block's first share: the sequence that holds it
+// and the work before that sequence.  `shared` has a row for each warp.
+struct Place {
+  int index;       // the batch's size when no sequence holds it
+  int64_t before;
+};
 
-// Item and offset in it of a position of a sequence's work.
-__device__ __forceinline__ void item_of(const Work& w, int64_t in, int* item, int* off) {
-  const int length = w.units + kItemUnits;
-  if (in < (int64_t(1) << 31)) {  // the common case: no 64-bit division
-    *item = int(unsigned(in) / unsigned(length));
-    *off = int(unsigned(in) - unsigned(*item) * unsigned(length));
+struct PlanShared {
+  int64_t total[kWarps];
+  float count[kWarps][kPieces];
+  Place found;
+};
+
+template <int ROWS>
+__device__ __forceinline__ Plan make_plan(const AttnArgs& a, PlanShared& sh, Place* place) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int shares = int(gridDim.x) * kWarps;
+  // Every thread takes a run of sequences; most calls have one at most for each.
+  const int run = (a.batch + kThreads - 1) / kThreads;
+  const int first = min(int(threadIdx.x) * run, a.batch), last = min(first + run, a.batch);
+  int64_t total = 0, items0 = 0;
+  int units0 = 0;
+  float count[kPieces] = {};  // exact up to 2^24, far above a grid
+  for (int b = last - 1; b >= first; --b) {
+    const Work w = work_of<ROWS>(a, b);
+    items0 = w.items, units0 = w.units;
+    total += w.items * (w.units + kItemUnits);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      count[i] += float(w.items) * float(max((w.units + (1 << i) - 1) >> i, 1));
+  }
+  auto sum = [&](int64_t v) {
+#pragma unroll
+    for (int d = 16; d; d /= 2) v += __shfl_xor_sync(~0u, v, d);
+    return v;
+  };
+  const int64_t warp_total = sum(total);
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+#pragma unroll
+    for (int d = 16; d; d /= 2) count[i] += __shfl_xor_sync(~0u, count[i], d);
+  }
+  if (lane == 0) {
+    sh.total[warp] = warp_total;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) sh.count[warp][i] = count[i];
+  }
+  __syncthreads();
+  int64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) all += sh.total[w];
+  Plan p;
+  p.piece = 0;
+  p.share = max(int64_t(kMinShare), all < (int64_t(1) << 31)
+                                        ? int64_t((unsigned(all) + shares - 1) / unsigned(shares))
+                                        : (all + shares - 1) / shares);
+#pragma unroll
+  for (int i = kPieces - 1; i >= 0; --i) {
+    float pieces = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) pieces += sh.count[w][i];
+    if (pieces <= float(shares) && int64_t(1 << i) <= p.share + kItemUnits) p.piece = 1 << i;
+  }
+  if (p.piece) p.share = 1;
+  // Running sum of the work as the plan counts it.
+  const int64_t pos = p.share * kWarps * blockIdx.x;
+  int64_t own = 0;
+  if (run <= 1) {
+    own = items0 * p.length(units0);
   } else {
-    *item = int(in / length);
-    *off = int(in - int64_t(*item) * length);
+    for (int b = first; b < last; ++b) {
+      const Work w = work_of<ROWS>(a, b);
+      own += w.items * p.length(w.units);
+    }
   }
+  int64_t v = own;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int64_t u = __shfl_up_sync(~0u, v, d);
+    if (lane >= d) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) sh.total[warp] = v;
+  if (threadIdx.x == 0) sh.found = Place{a.batch, 0};
+  __syncthreads();
+  int64_t before = v - own;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) before += w < warp ? sh.total[w] : 0;
+  if (pos >= before && pos < before + own) {
+    int b = first;
+    for (; b < last - 1; ++b) {
+      const Work w = work_of<ROWS>(a, b);
+      if (pos < before + w.items * p.length(w.units)) break;
+      before += w.items * p.length(w.units);
+    }
+    sh.found = Place{b, before};
+  }
+  __syncthreads();
+  *place = sh.found;
+  return p;
 }
 
-// All work of the call, [kv head][tile][units] of one sequence after the other,
-// in equal shares: one for each CTA of a grid that is resident at once.  A
-// share that begins or ends among an item's units leaves a partial result in
-// the workspace (at most two for a CTA), which q4_join brings together.
+// What a warp does at a time: units [u0, u1) of an item's part of the cache.
+struct Segment {
+  Seq s;
+  Span v;
+  int b, head, row0, rows;
+  int u0, u1;
+  int slot;  // place of its partial result in the workspace, -1: the result is whole
+};
+
+// An item that several shares have a piece of, for q4_join; rows = 0: none.  The
+// pieces are in the slots first, then 2 k for the shares k = first / 2 + 1 .. last.
+struct alignas(16) Joint {
+  int token, row0;    // the sequence's first query token, the tile's first row
+  int rows, head;
+  int first, last;
+};
+
+// A warp's way through its share.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, 2)
-    q4_attend(const __grid_constant__ AttnArgs a) {
-  extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ TileShared<D, NT> sh;
-  constexpr int kRows = 8 * NT;
-  asm volatile("griddepcontrol.launch_dependents;");
-  Place place;
-  int64_t share = 0;
-  const int64_t total = block_locate(
-      [&](int b) { return work_of<kRows>(a, b).total; }, a.batch,
-      [&](int64_t all) {
-        share = share_of(all, gridDim.x);
-        return share * blockIdx.x;
-      },
-      sh.scan, &sh.place, &place);
-  const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
-  if (begin >= end) return;
-  int b = place.index;
-  int64_t before = place.before, pos = begin;
-  while (pos < end && b < a.batch) {
-    const Work w = work_of<kRows>(a, b);
-    if (w.total == 0) {
-      ++b;
-      continue;
-    }
-    int item, off;
-    item_of(w, pos - before, &item, &off);
-    const int n = int(min(int64_t(w.units + kItemUnits - off), end - pos));
-    const int head = item / w.tiles, row0 = (item % w.tiles) * kRows;
-    const int rows = min(kRows, w.rows - row0);
-    // Units of this share; the item's first kItemUnits positions stand for none.
-    const int u0 = max(off - kItemUnits, 0), u1 = max(off + n - kItemUnits, 0);
-    if (w.units == 0) {
-      if (off == 0) store_nothing<T, D>(a, w.s, row0, rows, head);
-    } else if (u1 > u0) {
-      const Span v = span_of(a, w.s, row0, rows);
-      const bool whole = u0 == 0 && u1 == w.units;
-      attend_segment<T, D, NT>(a, sh, ring, b, w.s, v, row0, rows, head, min(u0, v.units),
-                               min(u1, v.units),
-                               whole ? -1 : 2 * int(blockIdx.x) + (pos == begin ? 0 : 1));
-    }
-    pos += n;
-    if (pos - before == w.total) {
-      before = pos;
-      ++b;
-    }
-  }
-}
+struct Walk {
+  Plan plan;
+  int64_t share;                    // its number
+  int64_t begin, pos, end, before;  // positions; before: the sequence's first
+  int b;
+  bool told;                        // that an item of several pieces begins in the share
 
-// The pieces of an item that starts at `start`: shares first .. last hold units
-// of it.  A share's piece is its first (even slot) where the share begins inside
-// the item or at its start.
-struct Pieces {
-  int64_t start, share, first, last;
-  __device__ __forceinline__ int64_t slot(int64_t k) const {
-    return 2 * k + (start > k * share ? 1 : 0);
+  __device__ __forceinline__ void put(const AttnArgs& a, int at, const Joint& joint) const {
+    if (threadIdx.x % 32 == 0) a.joints[at] = joint;
+  }
+
+  // The next segment with units; rows that see nothing are written on the way.
+  __device__ bool next(const AttnArgs& a, Segment& g) {
+    constexpr int kRows = 8 * NT;
+    while (pos < end && b < a.batch) {
+      const Work w = work_of<kRows>(a, b);
+      const int length = plan.length(w.units);
+      const int64_t in = pos - before, total = w.items * length;
+      if (in >= total) {
+        before += total;
+        ++b;
+        continue;
+      }
+      int item, off;
+      if (in < (int64_t(1) << 31)) {  // the common case: no 64-bit division
+        item = int(unsigned(in) / unsigned(length));
+        off = int(unsigned(in) - unsigned(item) * unsigned(length));
+      } else {
+        item = int(in / length);
+        off = int(in - int64_t(item) * length);
+      }
+      const int n = int(min(int64_t(length - off), end - pos));
+      const bool first = pos == begin;
+      pos += n;
+      g.head = item / w.tiles;
+      g.row0 = (item % w.tiles) * kRows;
+      g.rows = min(kRows, w.rows - g.row0);
+      if (w.units == 0) {
+        if (off == 0) {
+          store_nothing<T, D>(a, w.s, g.row0, g.rows, g.head);
+          if (a.joint_by_item) put(a, b * int(w.items) + item, Joint{});
+        }
+        continue;
+      }
+      const int u0 = plan.unit(w.units, off), u1 = plan.unit(w.units, off + n);
+      if (u1 <= u0) continue;
+      g.s = w.s;
+      g.b = b;
+      g.v = span_of(a, w.s, g.row0, g.rows);
+      g.slot = u0 == 0 && u1 == w.units ? -1 : int(2 * share) + (first ? 0 : 1);
+      g.u0 = min(u0, g.v.units);
+      g.u1 = min(u1, g.v.units);
+      if (u0 == 0) {  // the item's first piece: say who else has one
+        Joint joint{};
+        if (g.slot >= 0) {
+          const int64_t end_of = before + int64_t(item + 1) * length - 1;
+          joint = Joint{w.s.start, g.row0, g.rows, g.head, g.slot, int(end_of / plan.share)};
+        }
+        if (a.joint_by_item) put(a, b * int(w.items) + item, joint);
+        else if (g.slot >= 0) put(a, int(share), joint), told = true;
+      }
+      return true;
+    }
+    if (!a.joint_by_item && !told) {
+      put(a, int(share), Joint{});
+      told = true;
+    }
+    return false;
   }
 };
 
-__device__ __forceinline__ Pieces pieces_of(const Work& w, int64_t start, int64_t share) {
-  return Pieces{start, share, (start + kItemUnits) / share,
-                (start + kItemUnits + w.units - 1) / share};
+// ---- the kernel --------------------------------------------------------------
+
+// Where the units of a warp's next steps are, one in every lane: block id and
+// token run in the page.
+struct Units {
+  int id;
+  int within;  // -1: there is no such unit
+};
+
+// The 32 units from number i of the tile's on.
+__device__ __forceinline__ Units fetch_units(const AttnArgs& a, const Segment& g, int i) {
+  Units f{0, -1};
+  i += threadIdx.x % 32;
+  if (i < g.u1) {
+    const int n = i < g.v.sink_units ? i : i + g.v.gap;
+    const int page = a.upp_shift >= 0 ? n >> a.upp_shift : n / a.upp;
+    f.id = a.tables[int64_t(g.b) * a.table_stride + page];
+    f.within = n - page * a.upp;
+  }
+  return f;
 }
 
-// Joins one row's pieces, those of warp `part` of `parts`, in their order.
+// Queues the copies of a step's units, those of lanes `at` ..., into a stage:
+// 16-byte pieces lane, lane + 32, ... of each unit's codes, and one piece of the
+// runs of scales and zeros.  Returns which units are there.
 template <int D>
-__device__ __forceinline__ void join_row(const AttnArgs& a, const Pieces& p, int kRows, int r,
-                                         int part, int parts, float& m, float& l,
-                                         float4 (&o)[(D + 127) / 128]) {
+__device__ __forceinline__ uint32_t load_step(const AttnArgs& a, int head, const Units& f, int at,
+                                              uint32_t dst) {
+  using S = Shape<D>;
+  constexpr int kU = S::kUnits;
   const int lane = threadIdx.x % 32;
-  m = kNegInf;
-  for (int64_t k = p.first + lane; k <= p.last; k += 32)
-    m = fmaxf(m, a.part_ml[p.slot(k) * kRows + r].x);
+  // The four lanes with lane % kU = u look at unit u.
+  const int id = __shfl_sync(~0u, f.id, at + lane % kU);
+  const int within = __shfl_sync(~0u, f.within, at + lane % kU);
+  const bool real = within >= 0 && id >= 0 && id < a.cache.num_blocks;
+  if (!real && within >= 0) atomicExch(&g_q4_status, 5 /* KVX_ERR_BLOCK_ID */);
+  // A unit that is not there: its copies read nothing, from the first page.
+  const int64_t page = (real ? id : 0) * a.cache.stride + int64_t(head) * a.cache.head_bytes;
+  const int run = real ? within : 0;
+  const int64_t code = page + run * S::kUnit;
+  const uint32_t bits = __ballot_sync(~0u, real) & ((1u << kU) - 1u);
 #pragma unroll
-  for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+  for (int u = 0; u < kU; ++u) {
+    const int64_t offset = __shfl_sync(~0u, code, u) + 16 * lane;
+    const int size = (bits >> u) & 1u ? 16 : 0;
+#pragma unroll
+    for (int i = 0; i < S::kUnit / 512; ++i) {
+      // The pieces' places are permuted so that the fragments' reads meet no bank twice.
+      const int c = lane + 32 * i;
+      const int kc = D == 256 ? c ^ (4 * ((c >> 3) & 1)) : c;
+      const int vc = c ^ (D == 64    ? 2 * ((c >> 3) & 1)
+                          : D == 128 ? 2 * ((c >> 3) & 3)
+                                     : 2 * ((c >> 4) & 3));
+      copy16(dst + u * S::kUnit + 16 * kc, a.cache.pages[0] + offset + 512 * i, size);
+      copy16(dst + (kU + u) * S::kUnit + 16 * vc, a.cache.pages[1] + offset + 512 * i, size);
+    }
+  }
+  // Lane t * 4 kU + p * kU + u copies piece p of unit u's run of tensor t.
+  if (lane < 8 * kU)
+    copy16(dst + 2 * kU * S::kUnit + lane / (4 * kU) * S::kParams + 64 * (lane % kU) +
+               16 * (lane / kU % 4),
+           a.cache.pages[lane / (4 * kU) % 2] + page + a.cache.block_size * (D / 2) +
+               run * 64 + 16 * (lane / kU % 4),
+           real ? 16 : 0);
+  return bits;
+}
+
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// Writes a segment's result: a thread has D/8 dimensions of its columns' rows.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void store_segment(const AttnArgs& a, const Segment& seg,
+                                              WarpState<D, NT>& st) {
+  const int lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
+  const float back = st.c > 0.f ? 1.f / st.c : 0.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      // Sums over the tokens of the eight threads with this column.
+      float l = c ? st.l[n].y : st.l[n].x, z = st.z[n][c];
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) {
+        l += __shfl_xor_sync(~0u, l, d);
+        z += __shfl_xor_sync(~0u, z, d);
+      }
+      const int r = 8 * n + 2 * j + c;
+      if (r >= seg.rows) continue;
+      const float m = c ? -st.m[n].y : -st.m[n].x, mid = 7.5f * st.ps[n][c];
+      if (seg.slot >= 0 && g == 0)
+        a.part_ml[int64_t(seg.slot) * (8 * NT) + r] = make_float2(m, l);
+#pragma unroll
+      for (int d = 0; d < D / 16; d += 2) {
+        float4 o;
+        o.x = fmaf(fmaf(st.o[n][d][c], 16777216.f, -mid), back, z);
+        o.y = fmaf(fmaf(st.o[n][d][2 + c], 1048576.f, -mid), back, z);
+        o.z = fmaf(fmaf(st.o[n][d + 1][c], 16777216.f, -mid), back, z);
+        o.w = fmaf(fmaf(st.o[n][d + 1][2 + c], 1048576.f, -mid), back, z);
+        const int at = g * (D / 8) + 2 * d;
+        if (seg.slot >= 0)
+          *reinterpret_cast<float4*>(a.part_o + (int64_t(seg.slot) * (8 * NT) + r) * D + at) = o;
+        else
+          store_row<T>(a, seg.s, seg.row0 + r, seg.head, at, o, m, l);
+      }
+    }
+}
+
+// Each warp takes its share's segments one after the other, their units in
+// steps through its own ring of two cp.async stages; during a segment's last
+// step the next one's first is on its way already.  Segments that end or begin
+// inside an item leave a partial result in the workspace (at most two for a
+// warp), which q4_join brings together.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT))
+    q4_attend(const __grid_constant__ AttnArgs a) {
+  using S = Shape<D>;
+  constexpr int kRows = 8 * NT, kU = S::kUnits;
+  extern __shared__ __align__(128) uint8_t shared[];
+  __shared__ PlanShared plan_shared;
+  __shared__ uint2 fragments[NT == 1 ? 1 : kWarps][NT == 1 ? 1 : NT * (D / 16) * 32];
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  Walk<T, D, NT> walk;
+  {
+    Place place;
+    walk.plan = make_plan<kRows>(a, plan_shared, &place);
+    walk.b = place.index;
+    walk.before = place.before;
+    walk.share = int64_t(blockIdx.x) * kWarps + warp;
+    walk.begin = walk.pos = walk.plan.share * walk.share;
+    walk.end = walk.begin + walk.plan.share;
+    walk.told = false;
+  }
+  Segment seg, next;
+  if (!walk.next(a, seg)) return;
+  const uint32_t ring = uint32_t(__cvta_generic_to_shared(shared)) + warp * S::kWarpBytes;
+  const LaneAddress lane_at = lane_address<D>(ring, lane / 4, lane % 4);
+  uint32_t stage = 0, bits = 0;  // the step to take next: its stage, which of its units are there
+  bool loaded = false;           // its copies are on their way
+  Units now = fetch_units(a, seg, seg.u0), next_units{0, -1};
+  Fragments<D, NT> f;
+  f.shared = &fragments[NT == 1 ? 0 : warp][NT == 1 ? 0 : lane];
+  while (true) {
+    if (!loaded && seg.u0 < seg.u1) {
+      bits = load_step<D>(a, seg.head, now, 0, ring + stage);
+      commit();
+    }
+    loaded = false;
+    const bool more = walk.next(a, next);
+    if (more) next_units = fetch_units(a, next, next.u0);
+    Units later = fetch_units(a, seg, seg.u0 + 32);
+    Columns<NT> col;
+    load_queries<T, D, NT>(a, seg.s, seg.row0, seg.rows, seg.head, f, col);
+    WarpState<D, NT> st;
+    st.c = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      st.m[n] = make_float2(-kNegInf, -kNegInf), st.l[n] = make_float2(0.f, 0.f);
+      st.limit[n] = make_float2(kNegInf, kNegInf);
+      st.z[n][0] = st.z[n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        st.ps[n][i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) st.o[n][d][i] = 0.f;
+      }
+    }
+    // Units [plain_from, plain_to) need no mask: behind no row, and inside every
+    // row's window.
+    const Span& v = seg.v;
+    const int plain_from = max(v.sink_units, (max(v.p_hi - a.window + 1, 0) + 15) / 16 - v.gap);
+    const int plain_to = (v.p_lo + 1) / 16 - v.gap;
+    int at = 0;  // lane that has the step's first unit
+    for (int i = seg.u0; i < seg.u1; i += kU) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+      uint32_t next_bits = 0;
+      const uint32_t to = ring + (stage ^ uint32_t(S::kStage));
+      at = (at + kU) % 32;
+      if (i + kU < seg.u1) {
+        if (at == 0) {
+          now = later;
+          later = fetch_units(a, seg, i + kU + 32);
+        }
+        next_bits = load_step<D>(a, seg.head, now, at, to);
+      } else if (more && next.u0 < next.u1) {
+        next_bits = load_step<D>(a, next.head, next_units, 0, to);
+        loaded = true;
+      }
+      commit();
+      // Bits of the step's units that are there and need no mask.
+      const int low = min(max(plain_from - i, 0), kU), high = min(max(plain_to - i, 0), kU);
+      const uint32_t plain = bits & ((1u << high) - 1u) & ~((1u << low) - 1u);
+      attend_step<D, NT>(a, f, lane_at + stage, bits, plain, i, col, v, st);
+      __syncwarp();
+      stage ^= uint32_t(S::kStage);
+      bits = next_bits;
+    }
+    store_segment<T, D, NT>(a, seg, st);
+    if (!more) break;
+    seg = next;
+    now = next_units;
+  }
+}
+
+// ---- the join of partial results ---------------------------------------------
+
+// Weight of a piece with (maximum, sum) ml against the maximum m of all: a piece
+// without a finite score counts for nothing, unless a NaN is in it.
+__device__ __forceinline__ float piece_weight(float2 ml, float m) {
+  return ml.x == kNegInf ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - m);
+}
+
+// Sums the pieces part, part + parts, ... of eight >> kLg rows of a joint; what bounds
+// it is the latency of its loads, so a warp has eight rows' pieces in flight.
+// Slot q is row q & mask, piece q >> kLg' of a round.  Lane q has the row's m and l.
+template <int D, int kLg>
+__device__ __forceinline__ void join_pieces(const AttnArgs& a, const Joint& x, int kRows, int r0,
+                                            int rows, int part, int parts, float& m, float& l,
+                                            float4 (&o)[1 << kLg][(D + 127) / 128]) {
+  constexpr int kParts = (D + 127) / 128, kMask = (1 << kLg) - 1;
+  constexpr int kSlots = D == 256 ? 8 : 16, kPer = kSlots >> kLg;  // pieces of a round
+  const int lane = threadIdx.x % 32, count = x.last - x.first / 2 + 1;
+  auto slot = [&](int k) { return int64_t(k ? 2 * (x.first / 2 + k) : x.first) * kRows; };
+  const int r = r0 + min(lane & kMask, rows - 1);
+  m = kNegInf;
+  for (int k = lane >> kLg; k < count; k += 32 >> kLg) m = fmaxf(m, a.part_ml[slot(k) + r].x);
+#pragma unroll
+  for (int d = 1 << kLg; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
   l = 0.f;
 #pragma unroll
-  for (int i = 0; i < (D + 127) / 128; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int64_t k = p.first + part; k <= p.last; k += parts) {
-    const int64_t at = p.slot(k) * kRows + r;
-    const float2 ml = a.part_ml[at];
-    float4 x[(D + 127) / 128];
+  for (int q = 0; q <= kMask; ++q)
 #pragma unroll
-    for (int i = 0; i < (D + 127) / 128; ++i) {
-      const int d = 128 * i + 4 * lane;
-      x[i] = d < D ? *reinterpret_cast<const float4*>(a.part_o + at * D + d)
-                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < kParts; ++i) o[q][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = part * kPer; k0 < count; k0 += parts * kPer) {
+    const int mine = k0 + ((lane % kSlots) >> kLg);
+    const float2 ml = mine < count ? a.part_ml[slot(mine) + r] : make_float2(kNegInf, 0.f);
+    float4 v[kSlots][kParts];
+#pragma unroll
+    for (int q = 0; q < kSlots; ++q) {
+      const int row = r0 + min(q & kMask, rows - 1);
+      const float* from = a.part_o + (slot(min(k0 + (q >> kLg), count - 1)) + row) * D;
+#pragma unroll
+      for (int i = 0; i < kParts; ++i)
+        v[q][i] = 128 * i + 4 * lane < D
+                      ? *reinterpret_cast<const float4*>(from + 128 * i + 4 * lane)
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    // A piece without a finite score counts for nothing, unless a NaN is in it.
-    const float f = ml.x == kNegInf ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - m);
-    if (f != 0.f) {
-      l = fmaf(f, ml.y, l);
+    const float f = piece_weight(ml, m);
+    float add = f != 0.f ? f * ml.y : 0.f;
 #pragma unroll
-      for (int i = 0; i < (D + 127) / 128; ++i) {
-        o[i].x = fmaf(f, x[i].x, o[i].x), o[i].y = fmaf(f, x[i].y, o[i].y);
-        o[i].z = fmaf(f, x[i].z, o[i].z), o[i].w = fmaf(f, x[i].w, o[i].w);
+    for (int d = 1 << kLg; d < kSlots; d *= 2) add += __shfl_xor_sync(~0u, add, d);
+    l += add;
+#pragma unroll
+    for (int q = 0; q < kSlots; ++q) {
+      const float fq = __shfl_sync(~0u, f, q);
+      if (fq != 0.f) {  // what a piece without weight holds may be anything
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          float4& s = o[q & kMask][i];
+          s.x = fmaf(fq, v[q][i].x, s.x), s.y = fmaf(fq, v[q][i].y, s.y);
+          s.z = fmaf(fq, v[q][i].z, s.z), s.w = fmaf(fq, v[q][i].w, s.w);
+        }
       }
     }
   }
 }
 
-// Joins the partial results of items that several CTAs shared; the pieces are
-// summed in an order that does not vary.  Two forms:
-//   kByRow false: block k looks at the border behind share k and works when it
-//     is the first border among an item's units; a warp takes a row.
-//   kByRow true: a block for each row of each item, its warps share the pieces:
-//     for few items with many pieces, where a warp alone would take long.
-template <typename T, int D, int NT, bool kByRow>
-__global__ void __launch_bounds__(kThreads) q4_join(const __grid_constant__ AttnArgs a,
-                                                    int shares) {
-  __shared__ int64_t scan[kWarps];
-  __shared__ Place found;
-  __shared__ float4 part[kByRow ? kWarps : 1][(D + 127) / 128][32];
-  __shared__ float part_l[kWarps];
-  constexpr int kRows = 8 * NT;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  Place place;           // the item's sequence and the work before it
-  int64_t share = 0, start = 0;  // work before the item
-  bool none = false;
-  if constexpr (kByRow) {
-    // Few sequences: one thread walks them.
-    __shared__ int64_t walked[2];
-    if (threadIdx.x == 0) {
-      int64_t left = blockIdx.x / kRows, total = 0;
-      found = Place{a.batch, 0};
-      for (int b = 0; b < a.batch; ++b) {
-        const Work w = work_of<kRows>(a, b);
-        const int64_t items = int64_t(w.tiles) * a.cache.kv_heads;
-        if (left >= 0 && left < items) {
-          found = Place{b, total};
-          walked[1] = total + left * (w.units + kItemUnits);
-        }
-        left -= items;
-        total += w.total;
-      }
-      walked[0] = total;
-    }
-    __syncthreads();
-    place = found;
-    share = share_of(walked[0], shares);
-    start = walked[1];
-    none = place.index >= a.batch;
-  } else {
-    const int64_t total = block_locate(
-        [&](int b) { return work_of<kRows>(a, b).total; }, a.batch,
-        [&](int64_t all) {
-          share = share_of(all, shares);
-          return share * (int64_t(blockIdx.x) + 1);
-        },
-        scan, &found, &place);
-    start = share * (int64_t(blockIdx.x) + 1);  // the border, for now
-    none = start >= total;
-  }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (none) return;
-  const Work w = work_of<kRows>(a, place.index);
-  if (w.units == 0) return;
-  int item, off;
-  item_of(w, start - place.before, &item, &off);
-  start -= off;
-  const Pieces p = pieces_of(w, start, share);
-  if (p.first == p.last || (!kByRow && p.first != blockIdx.x)) return;
-  const int row0 = (item % w.tiles) * kRows, rows = min(kRows, w.rows - row0);
-  const int head = item / w.tiles;
+template <typename T, int D, int kLg>
+__device__ __forceinline__ void join_rows(const AttnArgs& a, const Joint& x, int kRows, int r0,
+                                          int rows) {
+  const int lane = threadIdx.x % 32;
   float m, l;
-  float4 o[(D + 127) / 128];
-  if (!kByRow) {
-    for (int r = warp; r < rows; r += kWarps) {
-      join_row<D>(a, p, kRows, r, 0, 1, m, l, o);
+  float4 o[1 << kLg][(D + 127) / 128];
+  join_pieces<D, kLg>(a, x, kRows, r0, rows, 0, 1, m, l, o);
 #pragma unroll
-      for (int i = 0; i < (D + 127) / 128; ++i)
-        if (128 * i + 4 * lane < D)
-          store_row<T>(a, w.s, row0 + r, head, 128 * i + 4 * lane, o[i], m, l);
-    }
-    return;
+  for (int q = 0; q < 1 << kLg; ++q) {
+    const float mq = __shfl_sync(~0u, m, q), lq = __shfl_sync(~0u, l, q);
+#pragma unroll
+    for (int i = 0; i < (D + 127) / 128; ++i)
+      if (q < rows && 128 * i + 4 * lane < D)
+        store_row<T>(a, Seq{x.token, 0, 0}, x.row0 + r0 + q, x.head, 128 * i + 4 * lane, o[q][i],
+                     mq, lq);
   }
-  const int r = blockIdx.x % kRows;
-  if (r >= rows) return;
-  join_row<D>(a, p, kRows, r, warp, kWarps, m, l, o);
-#pragma unroll
-  for (int i = 0; i < (D + 127) / 128; ++i) part[kByRow ? warp : 0][i][lane] = o[i];
-  if (lane == 0) part_l[warp] = l;
-  __syncthreads();
-  if (warp > 0) return;
-#pragma unroll
-  for (int k = 1; k < kWarps; ++k) {
-    l += part_l[k];
-#pragma unroll
-    for (int i = 0; i < (D + 127) / 128; ++i) {
-      const float4 x = part[kByRow ? k : 0][i][lane];
-      o[i].x += x.x, o[i].y += x.y, o[i].z += x.z, o[i].w += x.w;
+}
+
+// Joins the partial results of items that several warps shared; the pieces are
+// summed in an order that does not vary.  kByItem: a block for each row of each
+// item, its warps share the pieces; otherwise a warp for the item that begins in
+// a share, if one does.
+template <typename T, int D, int NT, bool kByItem>
+__global__ void __launch_bounds__(kJoinThreads) q4_join(const __grid_constant__ AttnArgs a,
+                                                        int shares) {
+  constexpr int kRows = 8 * NT, kParts = (D + 127) / 128;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if constexpr (!kByItem) {
+    const int at = blockIdx.x * kJoinWarps + warp;
+    if (at >= shares) return;
+    const Joint x = a.joints[at];
+    for (int r0 = 0; r0 < x.rows; r0 += 8) {
+      const int rows = min(8, x.rows - r0);
+      if (rows <= 1) join_rows<T, D, 0>(a, x, kRows, r0, rows);
+      else if (rows <= 2) join_rows<T, D, 1>(a, x, kRows, r0, rows);
+      else if (rows <= 4) join_rows<T, D, 2>(a, x, kRows, r0, rows);
+      else join_rows<T, D, 3>(a, x, kRows, r0, rows);
     }
-  }
+  } else {
+    __shared__ float4 part[kJoinWarps][kParts][32];
+    __shared__ float part_l[kJoinWarps];
+    const Joint x = a.joints[blockIdx.x / kRows];
+    const int r = blockIdx.x % kRows;
+    if (r >= x.rows) return;
+    float m, l;
+    float4 o[1][kParts];
+    join_pieces<D, 0>(a, x, kRows, r, 1, warp, kJoinWarps, m, l, o);
 #pragma unroll
-  for (int i = 0; i < (D + 127) / 128; ++i)
-    if (128 * i + 4 * lane < D)
-      store_row<T>(a, w.s, row0 + r, head, 128 * i + 4 * lane, o[i], m, l);
+    for (int i = 0; i < kParts; ++i) part[warp][i][lane] = o[0][i];
+    if (lane == 0) part_l[warp] = l;
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int k = 1; k < kJoinWarps; ++k) {
+      l += part_l[k];
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        const float4 v = part[k][i][lane];
+        o[0][i].x += v.x, o[0][i].y += v.y, o[0][i].z += v.z, o[0][i].w += v.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kParts; ++i)
+      if (128 * i + 4 * lane < D)
+        store_row<T>(a, Seq{x.token, 0, 0}, x.row0 + r, x.head, 128 * i + 4 * lane, o[0][i],
+                     m, __shfl_sync(~0u, l, 0));
+  }
 }
 
 }  // namespace q4
