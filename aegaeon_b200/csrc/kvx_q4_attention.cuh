@@ -1136,8 +1136,8 @@ __device__ __forceinline__ void join_rows(const AttnArgs& a, const Joint& x, int
 
 // Joins the partial results of items that several warps shared; the pieces are
 // summed in an order that does not vary.  kByItem: a block for each row of each
-// item, its warps share the pieces; otherwise a warp for the item that begins in
-// a share, if one does.
+// item, its warps share the pieces; otherwise the block's warps take the rows of
+// the items that begin in its shares.
 template <typename T, int D, int NT, bool kByItem>
 __global__ void __launch_bounds__(kJoinThreads) q4_join(const __grid_constant__ AttnArgs a,
                                                         int shares) {
@@ -1145,15 +1145,14 @@ __global__ void __launch_bounds__(kJoinThreads) q4_join(const __grid_constant__ 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if constexpr (!kByItem) {
-    const int at = blockIdx.x * kJoinWarps + warp;
-    if (at >= shares) return;
-    const Joint x = a.joints[at];
-    for (int r0 = 0; r0 < x.rows; r0 += 8) {
-      const int rows = min(8, x.rows - r0);
-      if (rows <= 1) join_rows<T, D, 0>(a, x, kRows, r0, rows);
-      else if (rows <= 2) join_rows<T, D, 1>(a, x, kRows, r0, rows);
-      else if (rows <= 4) join_rows<T, D, 2>(a, x, kRows, r0, rows);
-      else join_rows<T, D, 3>(a, x, kRows, r0, rows);
+    // Two rows at a time for a warp, so that eight of their pieces are in flight.
+    const int groups = min((a.group * (a.starts ? kRows : a.queries) + 1) / 2, kRows / 2);
+    for (int task = warp; task < kJoinWarps * groups; task += kJoinWarps) {
+      const int at = blockIdx.x * kJoinWarps + task / groups, r0 = 2 * (task % groups);
+      if (at >= shares) return;
+      const Joint x = a.joints[at];
+      if (x.rows - r0 >= 2) join_rows<T, D, 1>(a, x, kRows, r0, 2);
+      else if (x.rows > r0) join_rows<T, D, 0>(a, x, kRows, r0, 1);
     }
   } else {
     __shared__ float4 part[kJoinWarps][kParts][32];
