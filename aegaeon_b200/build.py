@@ -29,6 +29,7 @@ HEADERS = [
     os.path.join(HERE, "csrc", "kvx_kernels.cuh"),
     os.path.join(HERE, "csrc", "kvx_q4_rows.cuh"),
     os.path.join(HERE, "csrc", "kvx_q4_attention.cuh"),
+    os.path.join(HERE, "csrc", "kvx_q4_extend.cuh"),
     os.path.join(ROOT, "include", "kvx.h"),
 ]
 OUT = os.path.join(HERE, "libkvx.so")

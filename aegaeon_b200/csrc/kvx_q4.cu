@@ -10,6 +10,7 @@
 
 #include "../../include/kvx.h"
 #include "kvx_q4_attention.cuh"
+#include "kvx_q4_extend.cuh"
 #include "kvx_q4_rows.cuh"
 
 namespace kvx {
@@ -195,6 +196,28 @@ int launch_attention(const AttnArgs& a, int64_t head_dim, int rows, int grid, in
   return launch_attention<T, 256, 2>(a, grid, items, bound, device, s);
 }
 
+template <typename T, int D>
+int launch_extend(const AttnArgs& a, int64_t tiles, int device, cudaStream_t s) {
+  constexpr int shared = ExtendShape<D>::kShared;
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = cudaSuccess;
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(q4_extend<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    if (e != cudaSuccess) return cuda_fail("cudaFuncSetAttribute", e);
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  q4_extend<T, D><<<unsigned(tiles * a.cache.kv_heads), kExtendThreads, shared, s>>>(a, int(tiles));
+  e = cudaGetLastError();
+  return e == cudaSuccess ? KVX_OK : cuda_fail("q4_extend", e);
+}
+
+template <typename T>
+int launch_extend(const AttnArgs& a, int64_t head_dim, int64_t tiles, int device, cudaStream_t s) {
+  return head_dim == 64 ? launch_extend<T, 64>(a, tiles, device, s)
+                        : launch_extend<T, 128>(a, tiles, device, s);
+}
+
 }  // namespace
 
 // The device status word of this part (kvx_device_status reads all of them).
@@ -310,6 +333,7 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   a.o_token = out_token_stride;
   a.o_head = out_head_stride;
   a.o_vec = aligned(out, 8) && out_token_stride % 4 == 0 && out_head_stride % 4 == 0;
+  a.o_vec16 = aligned(out, 16) && out_token_stride % 8 == 0 && out_head_stride % 8 == 0;
   a.lse = lse;
   a.tables = block_tables;
   a.table_stride = table_stride;
@@ -328,6 +352,19 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   a.upp_shift = -1;
   for (int i = 0; i < 9; ++i)
     if (a.upp == 1 << i) a.upp_shift = i;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // Many rows: whole tiles of 128 rows on the tensor cores, where there are enough
+  // of them for half the SMs (they do not share a sequence's cache).
+  if (queries * group > 32 && head_dim <= 128 &&
+      num_tokens * group / kExtendRows * kv_heads >= sms / 2) {
+    const int64_t most = query_starts
+                             ? num_tokens * group / kExtendRows + batch
+                             : batch * ((queries * group + kExtendRows - 1) / kExtendRows);
+    if (most * kv_heads > INT32_MAX)
+      return fail(KVX_ERR_INVALID_ARGUMENT, "request too large for one call");
+    return dtype == kBf16 ? launch_extend<__nv_bfloat16>(a, head_dim, most, device, s)
+                          : launch_extend<__half>(a, head_dim, most, device, s);
+  }
   // CTAs: those that are resident at once, or fewer where even the longest
   // sequences that the tables can hold have too few units for their warps.
   const int64_t tiles = query_starts ? num_tokens * group / rows + batch
@@ -342,7 +379,6 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * head_dim);
   a.joints = reinterpret_cast<Joint*>(a.part_ml + pieces);
   a.joint_by_item = !query_starts && items <= kJoinByItem;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == kBf16 ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), items, bound, device, s)
                         : launch_attention<__half>(a, head_dim, rows, int(grid), items, bound, device, s);
 }

@@ -61,7 +61,8 @@ struct AttnArgs {
   int sinks;                // 0 without a window
   int upp;                  // 16-token units of a page
   int upp_shift;            // log2(upp), -1 when it is no power of two
-  int q_vec, o_vec;         // 16-byte accesses serve for query / out
+  int q_vec, o_vec;         // 16-byte accesses serve for query, 8-byte ones for out
+  int o_vec16;              // 16-byte ones for out
   float* part_o;            // [2 * shares][rows][D]
   float2* part_ml;          // [2 * shares][rows] (running maximum, sum)
   Joint* joints;            // [shares], or [items]

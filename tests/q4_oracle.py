@@ -51,8 +51,8 @@ def attention(query, key_pages, value_pages, tables, lens, starts=None, scale=No
         exp2 of the hardware adds 2^-21.  Weights are off by that, relatively,
         and the normalised sum by twice that times the largest |v|;
       * each weight is rounded once to fp16 before the product with the codes:
-        2^-11 of it, times |s (c - 7.5)| <= 7.5 s, since the sum of the rounded
-        weights is taken with the middle of the codes;
+        2^-11 of it, times |s (c - middle)| <= 8 s, since the middle of the codes
+        (7.5 or 8) is taken off them;
       * sums in 32 bits: n/8 + 64 roundings of 2^-24, each of at most the largest
         |s c| + |z|; their middle part cancels at most twice;
       * the output is rounded to its type: half a step.
@@ -80,29 +80,31 @@ def attention(query, key_pages, value_pages, tables, lens, starts=None, scale=No
         ids = tables[b][: -(-n // block)]
         at = lambda t: t[ids].transpose(0, 1).flatten(1, 2)[:, :n].double()  # noqa: E731
         kc, ks, kz, vc, vs, vz = (at(t) for t in (k_codes, k_s, k_z, v_codes, v_s, v_z))
-        for i, row in enumerate(rows):
-            p = n - len(rows) + i
-            j = torch.arange(n)
-            seen = j <= p
-            if window:
-                seen &= (j > p - window) | (j < sinks)
-            idx = torch.nonzero(seen)[:, 0]
-            if not len(idx):
-                continue
-            for h in range(heads):
-                kv = h // group
-                c, s, z = kc[kv][idx], ks[kv][idx, None], kz[kv][idx, None]
-                x = (c * s + z) @ q[row, h] * scale
-                size = ((c * s + z.abs()) @ q[row, h].abs()).max() * abs(scale)
-                dx = (dim / 16 + 4) * 2.0 ** -23 * size + 2.0 ** -21
-                w = torch.softmax(x, 0)
-                cv, sv, zv = vc[kv][idx], vs[kv][idx, None], vz[kv][idx, None]
-                v = cv * sv + zv
-                out[row, h] = w @ v
-                lse[row, h] = torch.logsumexp(x, 0)
-                most = (15 * sv + zv.abs()).max()
-                bound = 2 * dx * v.abs().max() + 2.0 ** -11 * 7.5 * (w @ sv[:, 0])
-                bound += 2 * (len(idx) / 8 + 64) * 2.0 ** -24 * most
-                out_bound[row, h] = bound + half * (out[row, h].abs() + bound) + 2.0 ** -25
-                lse_bound[row, h] = dx + 2.0 ** -22 * (lse[row, h].abs() + x.abs().max() + 1)
+        p = torch.arange(n - len(rows), n)[:, None]
+        j = torch.arange(n)[None]
+        seen = j <= p
+        if window:
+            seen &= (j > p - window) | (j < sinks)
+        some = seen.any(1)
+        for h in range(heads if n else 0):
+            kv = h // group
+            s, z, sv, zv = ks[kv][:, None], kz[kv][:, None], vs[kv], vz[kv]
+            k, v = kc[kv] * s + z, vc[kv] * sv[:, None] + zv[:, None]
+            x = q[rows.start:rows.stop, h] @ k.T * scale
+            size = q[rows.start:rows.stop, h].abs() @ (kc[kv] * s + z.abs()).T * abs(scale)
+            most = lambda t: torch.where(seen, t, torch.zeros(())).amax(1)  # noqa: E731
+            dx = (dim / 16 + 4) * 2.0 ** -23 * most(size) + 2.0 ** -21
+            x = torch.where(seen, x, -math.inf)
+            total = torch.logsumexp(x, 1)
+            w = torch.where(seen, torch.exp(x - total[:, None]), torch.zeros(()))
+            w[~some] = 0
+            o = w @ torch.where(seen.any(0)[:, None], v, torch.zeros(()))
+            bound = 2 * dx * most(v.abs().amax(1)[None].expand_as(x))
+            bound += 2.0 ** -11 * 8 * (w @ torch.where(seen.any(0), sv, torch.zeros(())))
+            bound += 2 * (seen.sum(1) / 8 + 64) * 2.0 ** -24 * most((15 * sv + zv.abs())[None].expand_as(x))
+            bound = bound[:, None]
+            out[rows.start:rows.stop, h] = o
+            lse[rows.start:rows.stop, h] = total
+            out_bound[rows.start:rows.stop, h] = bound + half * (o.abs() + bound) + 2.0 ** -25
+            lse_bound[rows.start:rows.stop, h] = dx + 2.0 ** -22 * (total.abs() + most(x.abs()) + 1)
     return out, lse, out_bound, lse_bound

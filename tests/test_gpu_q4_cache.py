@@ -270,6 +270,69 @@ def test_pieces_of_prompts(dim, group, block, window, sinks):
     assert (out[-6:] == 9).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,block,counts,lens", [
+    (32, 16, 128, 16, [340], [340]),                    # a whole prompt
+    (32, 16, 64, 32, [129, 0, 215], [500, 77, 215]),    # behind a prefix, none, whole
+    (28, 4, 128, 16, [350, 1, 64, 400], [363, 129, 70, 401]),
+    (16, 16, 128, 128, [640], [1000]),
+    (64, 8, 64, 48, [160, 5], [161, 3]),                # more queries than tokens
+])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (100, 4)])
+def test_many_rows(dtype, heads, kv_heads, dim, block, counts, lens, window, sinks):
+    """Enough rows for the tensor-core kernel (tiles of 128 rows for half the SMs)."""
+    assert sum(counts) * (heads // kv_heads) // 128 * kv_heads >= 74
+    kp, vp, tables, lengths, _ = make_cache(lens, kv_heads, dim, block, 55)
+    starts = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], device="cuda",
+                          dtype=torch.int32)
+    query = randn((sum(counts) + 3, heads, dim), dtype, 56)
+    out = torch.full_like(query, 9.0)
+    check(query, kp, vp, tables, lengths, starts, window=window, sinks=sinks, out=out)
+    assert (out[-3:] == 9).all()
+
+
+def test_many_rows_alike_and_strided():
+    """The same number of rows for every sequence, query and out inside wider
+    tensors, blocks that are not there, and the same result twice."""
+    kp, vp, tables, lengths, _ = make_cache([333, 0, 150], 8, 128, 16, 57)
+    wide = randn((3 * 110, 40, 136), torch.bfloat16, 58)
+    for q in (wide[:, 4:36, :128], wide[:, 4:36, 5:133]):
+        want = check(q, kp, vp, tables, lengths)
+        out = torch.full((330, 32, 137), 5.0, dtype=torch.bfloat16, device="cuda")
+        got = q4_cache.attention(q, kp, vp, tables, lengths, out=out[..., 1:129])
+        assert torch.equal(got, want[0])
+        assert (out[..., 0] == 5).all() and (out[..., 129:] == 5).all()
+    q = wide[:, 4:36, :128]
+    want = q4_cache.attention(q, kp, vp, tables, lengths)
+    assert torch.equal(want, q4_cache.attention(q, kp, vp, tables, lengths))
+    tables[0, 3] = -1
+    got = q4_cache.attention(q, kp, vp, tables, lengths)
+    assert _lib.device_status(0, reset=True) == _lib.KVX_ERR_BLOCK_ID
+    assert torch.isfinite(got).all() and not torch.equal(got[:110], want[:110])
+    assert torch.equal(got[110:], want[110:])
+
+
+def test_many_rows_scales_and_nan():
+    lens = [260]
+    kp, vp, tables, lengths, slots = make_cache(lens, 16, 128, 16, 59)
+    base = randn((170, 64, 128), torch.bfloat16, 60)
+    for factor in (1e-30, 40.0, 0.0):
+        check(base * factor, kp, vp, tables, lengths)
+    check(base, kp, vp, tables, lengths, scale=-0.3)
+    key = randn((260, 16, 128), torch.float32, 62)
+    value = randn((260, 16, 128), torch.float32, 63)
+    grow = torch.exp2(torch.linspace(-18, 13, 260, device="cuda"))[:, None, None]
+    for factor in (grow, grow.flip(0), torch.zeros_like(grow)):
+        q4_cache.write(key, value * factor, kp, vp, slots)
+        check(base, kp, vp, tables, lengths)
+    bad = torch.full((1, 16, 128), math.nan, device="cuda")
+    fine = torch.ones_like(bad)
+    for k, v in ((bad, fine), (fine, bad)):
+        q4_cache.write(k, v, kp, vp, slots[200:201])
+        got = q4_cache.attention(base, kp, vp, tables, lengths)
+        assert torch.isfinite(got[:110]).all() and got[110:].isnan().all()
+
+
 def test_lengths_that_the_shares_cut():
     """Long enough that many CTAs share a head, at lengths around their borders."""
     for n in (4095, 4096, 4097, 9000):
