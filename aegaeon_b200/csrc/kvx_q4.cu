@@ -356,7 +356,7 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   // Many rows: whole tiles of 128 rows on the tensor cores, where there are enough
   // of them for half the SMs (they do not share a sequence's cache).
   if (queries * group > 32 && head_dim <= 128 &&
-      num_tokens * group / kExtendRows * kv_heads >= sms / 2) {
+      num_tokens * group / kTileRows * kv_heads >= sms / 2) {
     const int64_t most = query_starts
                              ? num_tokens * group / kExtendRows + batch
                              : batch * ((queries * group + kExtendRows - 1) / kExtendRows);

@@ -340,6 +340,30 @@ def test_lengths_that_the_shares_cut():
         check(randn((1, 7, 128), torch.bfloat16, 61), kp, vp, tables, lengths)
 
 
+@pytest.mark.parametrize("batch", [129, 700])
+def test_more_sequences_than_threads(batch):
+    """A thread of the planning looks at several sequences; lengths from nothing up."""
+    lens = [(7 * i) % 90 for i in range(batch)]
+    lens[batch // 2] = 2000
+    kp, vp, tables, lengths, _ = make_cache(lens, 2, 64, 16, 65)
+    check(randn((batch, 4, 64), torch.float16, 66), kp, vp, tables, lengths)
+    counts = [min(n, i % 3) for i, n in enumerate(lens)]
+    starts = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], device="cuda",
+                          dtype=torch.int32)
+    check(randn((sum(counts), 4, 64), torch.bfloat16, 67), kp, vp, tables, lengths, starts,
+          window=30, sinks=2)
+
+
+def test_many_rows_of_many_sequences():
+    lens = [(11 * i) % 60 + 1 for i in range(1100)]
+    counts = [min(n, 20) for n in lens]
+    assert sum(counts) * 2 // 128 >= 74
+    kp, vp, tables, lengths, _ = make_cache(lens, 1, 64, 16, 68)
+    starts = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], device="cuda",
+                          dtype=torch.int32)
+    check(randn((sum(counts), 2, 64), torch.float16, 69), kp, vp, tables, lengths, starts)
+
+
 def test_scales_and_ranges():
     """Queries of any range, scores far apart, values of small and large scale."""
     lens = [200, 64]
