@@ -287,7 +287,8 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
                      void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
                      int dtype, int64_t num_tokens, int64_t num_heads, const void* key_pages,
                      const void* value_pages, int64_t page_stride, int64_t num_blocks,
-                     int64_t kv_heads, int64_t block_size, int64_t head_dim, const int32_t* block_tables, int64_t table_stride, int64_t table_width,
+                     int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                     const int32_t* block_tables, int64_t table_stride, int64_t table_width,
                      const int32_t* seq_lens, const int32_t* query_starts, int64_t batch,
                      double scale, int64_t window, int64_t sinks, void* workspace,
                      uint64_t workspace_bytes, void* stream) {
@@ -372,15 +373,16 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   const int64_t units = std::max<int64_t>(table_width * a.upp, 1);
   const int64_t items = tiles * kv_heads;
   int64_t grid = resident(rows, head_dim, sms);
-  const double bound = double(items) * double(units);
+  const double bound = double(items) * double((units + kPiece - 1) / kPiece);
   if (bound < double(grid * kWarps)) grid = (int64_t(bound) + kWarps - 1) / kWarps;
   const int64_t pieces = 2ll * kWarps * resident(rows, head_dim, sms) * rows;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * head_dim);
   a.joints = reinterpret_cast<Joint*>(a.part_ml + pieces);
   a.joint_by_item = !query_starts && items <= kJoinByItem;
-  return dtype == kBf16 ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), items, bound, device, s)
-                        : launch_attention<__half>(a, head_dim, rows, int(grid), items, bound, device, s);
+  return dtype == kBf16
+             ? launch_attention<__nv_bfloat16>(a, head_dim, rows, int(grid), items, bound, device, s)
+             : launch_attention<__half>(a, head_dim, rows, int(grid), items, bound, device, s);
 }
 
 }  // extern "C"

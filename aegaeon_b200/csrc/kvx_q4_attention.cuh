@@ -26,12 +26,16 @@ constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr int kNoWindow = 1 << 30;
 // What an item (a tile of query rows with one kv head) costs a warp besides its
-// 16-token units, in units: its queries, its first block ids, its result.
-constexpr int kItemUnits = 3;
+// 16-token units, in units: its queries, its first block ids, its result.  Measured
+// with 3 / 12 / 16 / 24: 16 requests of 1024 to 2048 tokens with 32 kv heads 38.4 /
+// 36.2 / 36.4 / 36.0 us, 128 of 4096 to 8192 with 8 170 / 166 / 164 / 168 us.
+constexpr int kItemUnits = 16;
 // Fewest units of a share when items are cut wherever shares end.
-constexpr int kMinShare = 8;
-// Sizes of the pieces that items may be cut into instead: 1 << 0 ... kPieces - 1.
-constexpr int kPieces = 6;
+constexpr int kMinShare = 24;
+// Units of the pieces that items may be cut into instead, kPiece << 0 ... kPieces - 1.
+// Below four a warp's step is not full, and there are more pieces to join (one
+// request of 1025 tokens: 10.7 us with single units, 10.3 with four).
+constexpr int kPiece = 4, kPieces = 4;
 // CTAs that an SM holds.
 __host__ __device__ constexpr int ctas_per_sm(int head_dim, int rows) {
   return head_dim == 256 && rows > 8 ? 1 : 2;
@@ -626,7 +630,7 @@ __device__ __forceinline__ void store_nothing(const AttnArgs& a, const Seq& s, i
 //   running: an item counts units + kItemUnits, and shares end wherever they do.
 // A warp works alone: no barrier, and short items cost it little.  (With a CTA's
 // four warps on one item and their results joined in shared memory, 16 requests
-// of 1024 to 2048 tokens with 32 kv heads took 42 us.)  What a call's sequences are
+// of 1024 to 2048 tokens with 32 kv heads took 42 us, 36 like this.)  What a call's sequences are
 // is known on the device only, so every CTA works the plan out from the lengths.
 struct Plan {
   int piece;      // 0: running
@@ -686,7 +690,8 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs& a, PlanShared& sh, Pla
     total += w.items * (w.units + kItemUnits);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
-      count[i] += float(w.items) * float(max((w.units + (1 << i) - 1) >> i, 1));
+      count[i] +=
+          float(w.items) * float(max((w.units + (kPiece << i) - 1) / (kPiece << i), 1));
   }
   auto sum = [&](int64_t v) {
 #pragma unroll
@@ -718,7 +723,8 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs& a, PlanShared& sh, Pla
     float pieces = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) pieces += sh.count[w][i];
-    if (pieces <= float(shares) && int64_t(1 << i) <= p.share + kItemUnits) p.piece = 1 << i;
+    if (pieces <= float(shares) && int64_t(kPiece << i) <= p.share + kItemUnits)
+      p.piece = kPiece << i;
   }
   if (p.piece) p.share = 1;
   // Running sum of the work as the plan counts it.
@@ -956,8 +962,11 @@ __device__ __forceinline__ void store_segment(const AttnArgs& a, const Segment& 
     }
 }
 
-// Each warp takes its share's segments one after the other, their units in
-// steps through its own ring of two cp.async stages; during a segment's last
+// What bounds it: the bytes of the cache where sequences are long (128 requests of
+// 4096 to 8192 tokens, 8 kv heads: 164 us, 5.25 TB/s, 81% of the card's copy rate;
+// 209 instructions for 16 tokens of a head, half of them unpacking), and what a
+// launch, an item and the join cost where they are short.  Each warp takes its
+// share's segments one after the other, their units in steps through its own ring of two cp.async stages; during a segment's last
 // step the next one's first is on its way already.  Segments that end or begin
 // inside an item leave a partial result in the workspace (at most two for a
 // warp), which q4_join brings together.
