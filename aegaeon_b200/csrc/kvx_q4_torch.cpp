@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -109,6 +110,12 @@ int check_rows(const at::Tensor& key, const at::Tensor& value, int64_t tokens,
   return kind;
 }
 
+// Whether two tensors share bytes, as far as their strides tell.
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  const at::MemOverlapStatus s = at::get_overlap_status(x, y);
+  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
+}
+
 int64_t check_slots(const at::Tensor& s, c10::Device device) {
   REQUIRE(s.scalar_type() == at::kLong && s.dim() == 1 && s.is_contiguous(),
           "slots must be a contiguous int64 tensor of one dimension");
@@ -193,6 +200,8 @@ PyObject* py_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                key.size(2));
   const int64_t tokens = check_slots(slots, c.device);
   const int kind = check_rows(key, value, tokens, c);
+  REQUIRE(!overlap(THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3])),
+          "key and value pages to write to must not overlap");
   if (tokens == 0) return PyLong_FromLong(0);
   return PyLong_FromLong(on_device(c.device, [&](void* stream) {
     return g_write(key.data_ptr(), value.data_ptr(), kind, tokens, key.stride(0), key.stride(1),
@@ -223,6 +232,7 @@ PyObject* py_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   } else {
     key = tensor(args[5], "out");
     value = tensor(args[6], "out");
+    REQUIRE(!overlap(key, value), "the key and value rows of out must not overlap");
   }
   const int kind = check_rows(key, value, tokens, c);
   int rc = 0;
@@ -306,6 +316,7 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     REQUIRE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() &&
                 out.device() == c.device && out.stride(2) == 1,
             "out must have the shape, type and device of query and contiguous rows");
+    REQUIRE(!overlap(out, q), "out must not overlap query: other warps still read it");
   }
   const int want_lse = PyObject_IsTrue(args[10]);
   if (want_lse < 0) return nullptr;

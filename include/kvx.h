@@ -386,7 +386,8 @@ int kvx_safetensors_meta_json(const char* file_path, char* out,
  * tokens j <= p, with window > 0 only those with j > p - window or j < sinks.
  * out: softmax(scale * q k) v, lse (optional, [num_tokens][num_heads]): the
  * natural log-sum-exp of the scores.  A row that sees nothing gives 0 and
- * -inf.  Rows behind the last sequence are left as they were.  workspace:
+ * -inf.  Rows behind the last sequence are left as they were.  out must not
+ * overlap query.  workspace:
  * kvx_q4_attention_workspace() bytes, 16-byte aligned, for this call alone
  * until it has finished; rows_per_sequence is the call's num_tokens (divided
  * by batch without query_starts) * num_heads / kv_heads.                       */

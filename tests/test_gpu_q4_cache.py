@@ -509,6 +509,28 @@ def test_other_stream_and_captured_graphs():
         assert torch.equal(outs[0], expect) and torch.equal(outs[1], expect)
 
 
+def test_first_call_of_a_kind_inside_a_capture():
+    """A call needs nothing outside the capture, not even a kernel's first (run alone,
+    this test is the first use of head_dim 256 with more than 8 rows)."""
+    kp, vp, tables, lengths, _ = make_cache([300, 40], 1, 256, 32, 135)
+    query = randn((2, 11, 256), torch.float16, 136)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = q4_cache.attention(query, kp, vp, tables, lengths)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, q4_cache.attention(query, kp, vp, tables, lengths))
+
+
+def test_many_heads_of_one_kv_head():
+    """128 query heads on one kv head: single tokens take the kernel of many rows
+    where there are sequences enough, the other one where there are not."""
+    for batch in (80, 3):
+        lens = [(37 * i) % 300 + 1 for i in range(batch)]
+        kp, vp, tables, lengths, _ = make_cache(lens, 1, 64, 16, 137)
+        check(randn((batch, 128, 64), torch.bfloat16, 138), kp, vp, tables, lengths)
+
+
 def test_nothing_to_do():
     kp, vp = q4_cache.allocate(2, 16, 2, 128)
     none = torch.zeros((0, 2, 128), dtype=torch.bfloat16, device="cuda")
@@ -535,7 +557,7 @@ def test_refusals_on_device_tensors():
                 dict(sinks=-1), dict(scale=float("nan")), dict(query=q.transpose(1, 2)),
                 dict(out=q.float()), dict(out=q[:1]), dict(query_starts=lengths),
                 dict(block_tables=tables.cpu()), dict(query=q.cpu()),
-                dict(query=torch.cat([q, q[:1]])), dict(key_pages=kp[..., :-1])):
+                dict(query=torch.cat([q, q[:1]])), dict(key_pages=kp[..., :-1]), dict(out=q)):
         with pytest.raises(ValueError):
             att(**bad)
     for bad in (dict(query=q.float()), dict(key_pages=kp.view(torch.int8))):
@@ -543,12 +565,16 @@ def test_refusals_on_device_tensors():
             att(**bad)
     rows, slots = randn((2, 2, 128), torch.bfloat16, 142), torch.arange(2, device="cuda")
     for bad in (dict(slots=slots.int()), dict(slots=slots[:1]), dict(slots=slots.cpu()),
-                dict(value=rows[:1]), dict(key=rows.transpose(0, 2))):
+                dict(value=rows[:1]), dict(key=rows.transpose(0, 2)), dict(value_pages=kp)):
         with pytest.raises(ValueError):
             q4_cache.write(**{**dict(key=rows, value=rows, key_pages=kp, value_pages=vp,
                                      slots=slots), **bad})
     with pytest.raises(TypeError):
         q4_cache.write(rows, rows.half(), kp, vp, slots)
+    with pytest.raises(ValueError, match="overlap"):
+        q4_cache.read(kp, vp, slots, head_dim=128, out=(rows, rows))
+    with pytest.raises(RuntimeError, match="gradient"):
+        q4_cache.write(rows.clone().requires_grad_(), rows, kp, vp, slots)
     with pytest.raises(TypeError):
         q4_cache.read(kp, vp, slots, head_dim=128, dtype=torch.float64)
 
