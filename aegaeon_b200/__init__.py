@@ -8,6 +8,7 @@ Modules:
   cache_transfer  extent arithmetic (aegaeon/cache_transfer.py)
   block_table     transfer planning (aegaeon/block_manager.py)
   switch          chunked weight upload overlapped with KV swap-in
+  q4_cache        a paged KV cache held in 4 bits: write, read, attention
   _lib            ctypes binding of libkvx.so (include/kvx.h)
 """
 

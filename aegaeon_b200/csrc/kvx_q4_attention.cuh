@@ -156,7 +156,6 @@ struct Shape {
   static constexpr int kStage = kUnits * 2 * kUnit + 2 * kParams;
   static constexpr int kWarpBytes = kStages * kStage;
   static constexpr int kShared = kWarps * kWarpBytes;
-  static constexpr int kKeyWords = D / 32;      // code words of a thread for one token of K
 };
 
 // First dimension of code word w of quad lane j in a K row.  At D = 256 the
@@ -1071,9 +1070,10 @@ __device__ __forceinline__ float piece_weight(float2 ml, float m) {
   return ml.x == kNegInf ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - m);
 }
 
-// Sums the pieces part, part + parts, ... of eight >> kLg rows of a joint; what bounds
-// it is the latency of its loads, so a warp has eight rows' pieces in flight.
-// Slot q is row q & mask, piece q >> kLg' of a round.  Lane q has the row's m and l.
+// Sums the pieces of 1 << kLg rows of a joint that fall to warp `part` of `parts`.  What
+// bounds it is the latency of its loads, so a warp has 16 (D = 256: 8) of them in
+// flight: slot q is row q & kMask of the piece q >> kLg further on.  Lane q has the
+// row's maximum and sum.
 template <int D, int kLg>
 __device__ __forceinline__ void join_pieces(const AttnArgs& a, const Joint& x, int kRows, int r0,
                                             int rows, int part, int parts, float& m, float& l,

@@ -2,7 +2,7 @@
 //
 // A decode turn calls write and attention once per layer, and the kernels of a
 // small batch take a few microseconds: checking the tensors in Python and
-// marshalling forty arguments through ctypes took 13 us a call.  This module does
+// marshalling their arguments through ctypes took 9 us a call more.  This module does
 // the checks on the C++ tensors, allocates the results and calls libkvx.so
 // through the addresses that bind() was given, so both routes reach the same
 // library instance.
