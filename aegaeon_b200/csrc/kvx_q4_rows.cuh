@@ -245,7 +245,8 @@ __device__ __forceinline__ uint2 codes_of(const T (&x)[16], float zero, float sc
   if (beyond || far > border) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float y = to_float(x[i]);
+      float y = to_float(x[i]);
+      if (clamped) y = fminf(fmaxf(y, -kLimit), kLimit);
       const uint32_t was = (w[i / 8] >> (4 * (i % 8))) & 15u;
       if (!beyond && fabsf(fmaf(-float(was), scale, y - zero)) <= border) continue;
       uint32_t c = was;
