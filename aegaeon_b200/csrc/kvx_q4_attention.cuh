@@ -10,8 +10,12 @@
 // code * 2^-24 (and 2^-20 one nibble further up), exact in the matrix
 // instruction's products; the powers of two leave with the epilogue.
 //
-// The running maximum is kept in powers of two and follows only when a score
-// passes it by 2^8, so that most tiles neither reduce it nor rescale.
+// p_j s'_j goes to the matrix instruction in fp16.  So a row's reference point follows
+// its largest p_j s'_j, not its largest p_j: a token of large scale that has no
+// weight then takes no bits from the others.  p_j itself stays in 32 bits, where
+// it may be as large as the scales are apart.  The reference point is kept in powers
+// of two and moves only when a product passes it by 2^8, so that most tiles
+// neither reduce it nor rescale.
 #pragma once
 
 #include "kvx_q4_rows.cuh"
@@ -260,15 +264,25 @@ __device__ __forceinline__ void load_queries(const AttnArgs& a, const Seq& s, in
   }
 }
 
+// log2 of a V scale, from its bits: at most 0.09 below it, which is enough to place
+// the reference point.  A row of one value has scale 0 and counts 2^-32, so that its
+// p is 2^46 at most.
+__device__ __forceinline__ float size_of(float scale) {
+  const float bits = __int2float_rn(int(__float_as_uint(scale) & 0x7fffffffu));
+  return fmaxf(fmaf(bits, 1.1920928955078125e-7f, -127.f), -32.f);
+}
+// Where the reference point is put above or below the largest product, in powers of
+// two, and how far above it a product may come: below 2^14.1 in all, inside fp16.
+constexpr float kLift = 6.f, kSlack = 8.f;
+
 // One warp's state over the units that it takes.
 template <int D, int NT>
 struct WarpState {
-  float o[NT][D / 16][4];  // sum of p * s * C * code, dimensions as in value_dim()
-  float ps[NT][4];         // sum of the same weights as the matrix instruction saw them
-  float2 m[NT], l[NT];     // minus the reference point, sum of the weights, by column
-  float2 limit[NT];        // raw score that moves the reference point
+  float o[NT][D / 16][4];  // sum of p * s * code, dimensions as in value_dim()
+  float ps[NT][4];         // sum of the same products as the matrix instruction saw them
+  float2 m[NT], l[NT];     // minus the reference point, sum of p, by column
+  float2 limit[NT];        // log2(p s) that moves the reference point; -inf: there is none yet
   float z[NT][2];          // sum of p * (zero + 7.5 scale)
-  float c;                 // C: power of two on the V scales, so that weights suit fp16
 };
 
 template <int kOffset>
@@ -430,7 +444,7 @@ template <int D, int NT, int U, int kAb, bool kMasked>
 __device__ __forceinline__ void attend_units(const AttnArgs& a, const Fragments<D, NT>& f,
                                              const LaneAddress& at,
                                              const int* number, const Columns<NT>& col,
-                                             const Span& v, WarpState<D, NT>& st) {
+                                             WarpState<D, NT>& st) {
   const int lane = threadIdx.x % 32, g = lane / 4;
   float x[kAb][NT][4];
   // (scale, zero) of tokens g and g + 8 of each unit: K, then V.
@@ -442,21 +456,21 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const Fragments<
     vp[u][1] = lds32<Shape<D>::kParams + at_u + 32>(at.p);
     unit_scores<D, NT, U + u>(at, f, x[u]);
   });
-  float vs[kAb][2], vz[kAb][2], most = 0.f;
+  float vs[kAb][2], vz[kAb][2], top[NT][2];  // top: largest log2(p s)
+#pragma unroll
+  for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = kNegInf;
 #pragma unroll
   for (int u = 0; u < kAb; ++u) {
-    float part[2];
+    float2 size[NT][2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float2 k = half2_at(kp[u][r]), w = half2_at(vp[u][r]);
-      vs[u][r] = part[r] = w.x;
+      vs[u][r] = w.x;
       vz[u][r] = fmaf(7.5f, w.x, w.y);
+      const float scale = size_of(w.x);
       const int unit = kMasked ? number[u] : 0, t = unit * 16 + g + 8 * r;
-      // Only of tokens that some row sees: what lies behind a sequence may be anything.
-      if (kMasked && !(unit >= 0 && t <= v.p_hi && (t > v.p_lo - a.window || t < a.sinks)))
-        part[r] = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float& y = x[u][n][2 * r + c];
@@ -467,55 +481,46 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const Fragments<
             y = seen ? y : kNegInf;
           }
         }
+        size[n][r] = fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]), col.factor[n],
+                          both(scale));
+      }
     }
-    most = max_abs(most, part[0], part[1]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      top[n][0] = max3(top[n][0], size[n][0].x, size[n][1].x);
+      top[n][1] = max3(top[n][1], size[n][0].y, size[n][1].y);
+    }
   }
-  // Move the reference point where a score passes it by 2^8, or the weights
-  // would leave fp16.  The factors are positive, so raw scores have the order.
-  float top[NT][2];
-  bool move = !(most * st.c <= 64.f);
+  bool move = false;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      top[n][c] = fmaxf(x[0][n][c], x[0][n][2 + c]);
-#pragma unroll
-      for (int u = 1; u < kAb; ++u) top[n][c] = max3(top[n][c], x[u][n][c], x[u][n][2 + c]);
-    }
+  for (int n = 0; n < NT; ++n)
     move |= top[n][0] > st.limit[n].x || top[n][1] > st.limit[n].y;
-  }
   if (__any_sync(~0u, move)) {
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-    float ratio = 1.f;
-    if (st.c == 0.f || !(most * st.c <= 64.f)) {
-      // most * C in [32, 64)
-      const uint32_t e = __float_as_uint(most) >> 23;
-      const float c = most > 0.f ? __uint_as_float((259u - e) << 23) : 16777216.f;
-      ratio = st.c == 0.f ? 1.f : c / st.c;
-      st.c = c;
-    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float by[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float factor = c ? col.factor[n].y : col.factor[n].x;
         float& m = c ? st.m[n].y : st.m[n].x;
-        float t = fmaxf(top[n][c] * factor, -m);
+        float& limit = c ? st.limit[n].y : st.limit[n].x;
+        float t = fmaxf(top[n][c], limit - kSlack);
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
-        by[c] = t == kNegInf ? 1.f : ex2(-m - t);
-        m = -t;
-        (c ? st.limit[n].y : st.limit[n].x) = (t + 8.f) / factor;
+        by[c] = 1.f;
+        if (t != kNegInf) {
+          t = ceilf(t);
+          if (limit != kNegInf) by[c] = ex2(kLift - t - m);
+          m = kLift - t;
+          limit = t + kSlack;
+        }
       }
       st.l[n].x *= by[0], st.l[n].y *= by[1];
       st.z[n][0] *= by[0], st.z[n][1] *= by[1];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        st.ps[n][i] *= by[i % 2] * ratio;
+        st.ps[n][i] *= by[i % 2];
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) st.o[n][d][i] *= by[i % 2] * ratio;
+        for (int d = 0; d < D / 16; ++d) st.o[n][d][i] *= by[i % 2];
       }
     }
   }
@@ -524,18 +529,12 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const Fragments<
   for (int u = 0; u < kAb; ++u)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float weight = vs[u][r] * st.c;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float2 m = st.m[n];
-        if (kMasked) {
-          m.x = m.x == -kNegInf ? 0.f : m.x;
-          m.y = m.y == -kNegInf ? 0.f : m.y;
-        }
-        float2 p = fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]), col.factor[n], m);
+        float2 p = fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]), col.factor[n], st.m[n]);
         p.x = ex2(p.x), p.y = ex2(p.y);
         st.l[n] = add2(st.l[n], p);
-        float y[2] = {p.x * weight, p.y * weight};
+        float y[2] = {p.x * vs[u][r], p.y * vs[u][r]};
         float z[2] = {fmaf(p.x, vz[u][r], st.z[n][0]), fmaf(p.y, vz[u][r], st.z[n][1])};
         if (kMasked) {  // a hidden token's scale and zero may be anything
           if (p.x == 0.f) y[0] = 0.f, z[0] = st.z[n][0];
@@ -565,7 +564,7 @@ __device__ __forceinline__ void attend_step(const AttnArgs& a, const Fragments<D
   constexpr uint32_t kAll = (1u << kU) - 1u;
   if constexpr (NT == 1 && kU == 4) {
     if (plain == kAll) {
-      attend_units<D, NT, 0, 4, false>(a, f, at, nullptr, col, v, st);
+      attend_units<D, NT, 0, 4, false>(a, f, at, nullptr, col, st);
       return;
     }
   }
@@ -574,7 +573,7 @@ __device__ __forceinline__ void attend_step(const AttnArgs& a, const Fragments<D
   each<kU / kAb>([&](auto index) {
     constexpr int kFirst = decltype(index)::value * kAb;
     if (((plain >> kFirst) & kPart) == kPart) {
-      attend_units<D, NT, kFirst, kAb, false>(a, f, at, nullptr, col, v, st);
+      attend_units<D, NT, kFirst, kAb, false>(a, f, at, nullptr, col, st);
     } else if ((there >> kFirst) & kPart) {
       int number[kAb];
 #pragma unroll
@@ -582,9 +581,18 @@ __device__ __forceinline__ void attend_step(const AttnArgs& a, const Fragments<D
         const int k = i + kFirst + u;
         number[u] = (there >> (kFirst + u)) & 1u ? (k < v.sink_units ? k : k + v.gap) : -1;
       }
-      attend_units<D, NT, kFirst, kAb, true>(a, f, at, number, col, v, st);
+      attend_units<D, NT, kFirst, kAb, true>(a, f, at, number, col, st);
     }
   });
+}
+
+// Natural logarithm of 2^m l; m is whole.  l's own power of two joins m first: both may
+// be large where the result is not.
+__device__ __forceinline__ float log_sum(float m, float l) {
+  if (l == 0.f) return kNegInf;
+  int e;
+  const float part = frexpf(l, &e);
+  return ((m + float(e)) + log2f(part)) * 0.6931471805599453f;
 }
 
 // Four dimensions of one row's result: sum / l and log-sum-exp; zeros and -inf
@@ -607,8 +615,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const Seq& s, int r
     for (int i = 0; i < 4; ++i) to[i] = x[i];
   }
   if (a.lse && d == 0)
-    a.lse[token * (int64_t(a.cache.kv_heads) * a.group) + h] =
-        l == 0.f ? kNegInf : (m + log2f(l)) * 0.6931471805599453f;
+    a.lse[token * (int64_t(a.cache.kv_heads) * a.group) + h] = log_sum(m, l);
 }
 
 // Rows of a tile that see nothing.
@@ -928,7 +935,6 @@ template <typename T, int D, int NT>
 __device__ __forceinline__ void store_segment(const AttnArgs& a, const Segment& seg,
                                               WarpState<D, NT>& st) {
   const int lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
-  const float back = st.c > 0.f ? 1.f / st.c : 0.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -942,16 +948,17 @@ __device__ __forceinline__ void store_segment(const AttnArgs& a, const Segment& 
       }
       const int r = 8 * n + 2 * j + c;
       if (r >= seg.rows) continue;
-      const float m = c ? -st.m[n].y : -st.m[n].x, mid = 7.5f * st.ps[n][c];
+      const bool none = (c ? st.limit[n].y : st.limit[n].x) == kNegInf;
+      const float m = none ? kNegInf : c ? -st.m[n].y : -st.m[n].x, mid = 7.5f * st.ps[n][c];
       if (seg.slot >= 0 && g == 0)
         a.part_ml[int64_t(seg.slot) * (8 * NT) + r] = make_float2(m, l);
 #pragma unroll
       for (int d = 0; d < D / 16; d += 2) {
         float4 o;
-        o.x = fmaf(fmaf(st.o[n][d][c], 16777216.f, -mid), back, z);
-        o.y = fmaf(fmaf(st.o[n][d][2 + c], 1048576.f, -mid), back, z);
-        o.z = fmaf(fmaf(st.o[n][d + 1][c], 16777216.f, -mid), back, z);
-        o.w = fmaf(fmaf(st.o[n][d + 1][2 + c], 1048576.f, -mid), back, z);
+        o.x = fmaf(st.o[n][d][c], 16777216.f, -mid) + z;
+        o.y = fmaf(st.o[n][d][2 + c], 1048576.f, -mid) + z;
+        o.z = fmaf(st.o[n][d + 1][c], 16777216.f, -mid) + z;
+        o.w = fmaf(st.o[n][d + 1][2 + c], 1048576.f, -mid) + z;
         const int at = g * (D / 8) + 2 * d;
         if (seg.slot >= 0)
           *reinterpret_cast<float4*>(a.part_o + (int64_t(seg.slot) * (8 * NT) + r) * D + at) = o;
@@ -1011,10 +1018,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT))
     Columns<NT> col;
     load_queries<T, D, NT>(a, seg.s, seg.row0, seg.rows, seg.head, f, col);
     WarpState<D, NT> st;
-    st.c = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      st.m[n] = make_float2(-kNegInf, -kNegInf), st.l[n] = make_float2(0.f, 0.f);
+      st.m[n] = st.l[n] = make_float2(0.f, 0.f);
       st.limit[n] = make_float2(kNegInf, kNegInf);
       st.z[n][0] = st.z[n][1] = 0.f;
 #pragma unroll

@@ -63,3 +63,185 @@ def test_codes_of_clamped_rows_follow_the_definition(dim):
         want = q4_oracle.quantise(x[:, 0])
         assert torch.equal(scale, want[1][:, 0]) and torch.equal(zero, want[2][:, 0])
         assert torch.equal(codes, want[0])
+
+
+# ---- value scales far apart ---------------------------------------------------------
+
+
+def attention_bound(query, kp, vp, tables, lens, starts=None, window=None, sinks=0):
+    """(out, bound) from the definition, where every term of the bound carries its
+    token's weight, so that what nobody attends to allows no error.
+
+    With w the weights (sum 1), s and z the value scales and zeros:
+      * a weight is off by dx, relatively: the score's (dim/16 + 4) 2^-23 max_j sum_d
+        |q_d| (s c_d + |z|) scale (products summed in 32 bits in dim/16 steps, three
+        more roundings, whole steps because an accumulation may truncate) and the
+        hardware's exp2, 2^-21.  The normalised sum moves by at most
+        2 dx sum_j w_j |v_j - out|;
+      * each product w_j s_j is rounded once to fp16: 2^-11 of it, times the
+        distance of a code from the middle, at most 8.  The largest product lies above 2^5
+        before that rounding, so those below fp16's normal numbers are off by 2^-25 each, 2^-30
+        of the largest; twice, since they may be scaled once more;
+      * n/8 + 64 roundings of 2^-24 in sums of w_j (15 s_j + |z_j|), doubled for the part of
+        the middle, which cancels;
+      * the rounding to the output's type, and fp16's smallest half step.
+    """
+    tokens, heads, dim = query.shape
+    group = heads // kp.shape[1]
+    q = query.double().cpu()
+    parts = [*q4_oracle.split(kp, dim), *q4_oracle.split(vp, dim)]
+    block = parts[0].shape[2]
+    lens, tables = lens.tolist(), tables.tolist()
+    per = tokens // len(lens)
+    starts = [i * per for i in range(len(lens) + 1)] if starts is None else starts.tolist()
+    out = torch.zeros(tokens, heads, dim, dtype=torch.float64)
+    bound = torch.zeros_like(out)
+    half = torch.finfo(query.dtype).eps / 2
+    for b, n in enumerate(lens):
+        lo, hi = starts[b], starts[b + 1]
+        ids = tables[b][: -(-n // block)]
+        kc, ks, kz, vc, vs, vz = (t[ids].transpose(0, 1).flatten(1, 2)[:, :n].double() for t in parts)
+        p, j = torch.arange(n - (hi - lo), n)[:, None], torch.arange(n)[None]
+        seen = j <= p
+        if window:
+            seen &= (j > p - window) | (j < sinks)
+        for h in range(heads):
+            kv = h // group
+            x = q[lo:hi, h]
+            k, v = kc[kv] * ks[kv][:, None] + kz[kv][:, None], vc[kv] * vs[kv][:, None] + vz[kv][:, None]
+            score = (x @ k.T / math.sqrt(dim)).masked_fill(~seen, -math.inf)
+            size = x.abs() @ (kc[kv] * ks[kv][:, None] + kz[kv].abs()[:, None]).T / math.sqrt(dim)
+            dx = (dim / 16 + 4) * 2.0 ** -23 * size.masked_fill(~seen, 0).amax(1) + 2.0 ** -21
+            w = torch.softmax(score, 1)
+            o = w @ v
+            spread = torch.stack([w[i] @ (v - o[i]).abs() for i in range(hi - lo)])
+            step = w * vs[kv]
+            e = 2 * dx[:, None] * spread
+            e = e + (8 * 2.0 ** -11 * step.sum(1) + 8 * n * 2.0 ** -29 * step.amax(1))[:, None]
+            e = e + (2 * (n / 8 + 64) * 2.0 ** -24 * (w @ (15 * vs[kv] + vz[kv].abs())))[:, None]
+            out[lo:hi, h] = o
+            bound[lo:hi, h] = e + half * (o.abs() + e) + (2.0 ** -25 if query.dtype is torch.float16 else 0)
+    return out, bound
+
+
+def steered_cache(lens, special, kv_heads, dim, block, small, seed):
+    """A cache whose values have the scale `small` but for single tokens.  special:
+    {(sequence, token): (push, rows)}: the key is -push in 16 channels where the queries are
+    about 2, and `rows` is the token's value row."""
+    need = [-(-n // block) for n in lens]
+    shape = (sum(need) + 1, kv_heads, q4_cache.head_bytes(block, dim))
+    kp, vp = (torch.full(shape, 0xFF, dtype=torch.uint8, device="cuda") for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    order = torch.randperm(shape[0], generator=g, device="cuda")
+    tables = torch.zeros((len(lens), max(need)), dtype=torch.int32, device="cuda")
+    at = 0
+    for b, n in enumerate(lens):
+        ids = order[at:at + need[b]]
+        at += need[b]
+        tables[b, :need[b]] = ids.int()
+        j = torch.arange(n, device="cuda")
+        key = randn((n, kv_heads, dim), torch.float32, seed + 2 * b + 1)
+        # a row's values step through the sixteen codes: scale `small`, exact
+        value = (torch.randint(0, 16, (n, kv_heads, dim), generator=g, device="cuda") - 7.5) * small
+        value[..., 0], value[..., 1] = -7.5 * small, 7.5 * small
+        for (seq, token), (push, rows) in special.items():
+            if seq == b:
+                key[token] = 0
+                key[token, :, :16] = -push
+                value[token] = rows
+        q4_cache.write(key, value, kp, vp, ids[j // block] * block + j % block)
+    return kp, vp, tables, torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+def steered_queries(tokens, heads, dim, dtype, seed):
+    q = randn((tokens, heads, dim), torch.float32, seed)
+    q[..., :16] = 2 + 0.1 * q[..., :16]
+    return q.to(dtype)
+
+
+def hold(query, kp, vp, tables, lens, starts=None, **kw):
+    got = q4_cache.attention(query, kp, vp, tables, lens, query_starts=starts, **kw).double().cpu()
+    want, bound = attention_bound(query, kp, vp, tables, lens, starts, **kw)
+    off = (got - want).abs()
+    assert (off <= bound).all(), f"off by {(off / bound.clamp(min=1e-30)).max()} bounds"
+
+
+def wide_row(scale, dim):
+    """A value row with that scale: all codes appear."""
+    return (torch.arange(dim, device="cuda") % 16 - 7.5) * scale
+
+
+# Scales of the token that nobody attends to (weight about 1e-18) and of the others.
+FAR_SCALES = [(0, -14), (4, -17), (10, -14), (13, -14), (13, -17)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("large,small", FAR_SCALES)
+@pytest.mark.parametrize("heads,kv_heads,dim,block", [
+    (4, 2, 64, 16), (7, 1, 128, 16), (12, 1, 128, 32), (32, 1, 128, 16), (4, 4, 256, 16), (12, 1, 256, 16)])
+def test_decode_with_a_far_value_scale(dtype, large, small, heads, kv_heads, dim, block):
+    """Wherever the token is: in the first unit, behind others, in the last one."""
+    lens = [100, 200, 333]
+    row = wide_row(2.0 ** large, dim)
+    special = {(0, 0): (15.0, row), (1, 111): (15.0, row), (2, 331): (15.0, row)}
+    cache = steered_cache(lens, special, kv_heads, dim, block, 2.0 ** small, 10)
+    hold(steered_queries(len(lens), heads, dim, dtype, 20), *cache)
+
+
+def test_far_value_scales_in_the_parts_of_a_long_sequence():
+    """Pieces of one sequence, with and without such a token, that are joined."""
+    row = wide_row(2.0 ** 13, 128)
+    special = {(0, 5): (15.0, row), (0, 3000): (15.0, row), (0, 4998): (15.0, row)}
+    cache = steered_cache([5000], special, 1, 128, 16, 2.0 ** -14, 30)
+    for dtype in DTYPES:
+        hold(steered_queries(1, 7, 128, dtype, 31), *cache)
+
+
+@pytest.mark.parametrize("large,small", FAR_SCALES)
+def test_a_scale_that_only_other_rows_see(large, small):
+    """Several queries share a tile; the last token is seen by the last of them alone."""
+    row = wide_row(2.0 ** large, 128)
+    lens = [60, 160]
+    cache = steered_cache(lens, {(0, 59): (15.0, row), (1, 157): (0.0, row)}, 2, 128, 16,
+                          2.0 ** small, 40)
+    hold(steered_queries(8, 6, 128, torch.float16, 41), *cache)
+    hold(steered_queries(8, 6, 128, torch.bfloat16, 42), *cache, window=30, sinks=3)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("large,small", FAR_SCALES)
+def test_many_rows_with_a_far_value_scale(large, small, dim):
+    """The kernel of many rows: rows that see the token and rows that do not."""
+    heads, kv_heads, lens, counts = 32, 16, [340, 300], [340, 150]
+    assert sum(counts) * (heads // kv_heads) // 128 * kv_heads >= 74
+    row = wide_row(2.0 ** large, dim)
+    special = {(0, 0): (15.0, row), (0, 200): (15.0, row), (1, 140): (15.0, row),
+               (1, 299): (0.0, row)}
+    cache = steered_cache(lens, special, kv_heads, dim, 16, 2.0 ** small, 50)
+    starts = torch.tensor([0, 340, 490], dtype=torch.int32, device="cuda")
+    hold(steered_queries(490, heads, dim, torch.float16, 51), *cache, starts=starts)
+    hold(steered_queries(490, heads, dim, torch.bfloat16, 52), *cache, starts=starts, window=90, sinks=2)
+
+
+@pytest.mark.parametrize("push", [-5.0, 0.0])
+def test_a_token_without_values_that_takes_the_weight(push):
+    """A row of zeros with nearly all of the weight (push -5: 1 - 2^-16 of it): what is left
+    of the other tokens is the whole output."""
+    zero = torch.zeros(128, device="cuda")
+    cache = steered_cache([150, 40], {(0, 0): (push, zero), (1, 20): (push, zero)}, 1, 128, 16, 1.0, 60)
+    hold(steered_queries(2, 7, 128, torch.bfloat16, 61), *cache)
+    cache = steered_cache([320], {(0, 0): (push, zero)}, 16, 128, 16, 1.0, 62)
+    hold(steered_queries(320, 32, 128, torch.bfloat16, 63), *cache)
+
+
+def test_log_sum_exp_with_any_value_scale():
+    """The log-sum-exp does not depend on the values.  Bound: the score's error, and
+    one rounding of the result's size, in a logarithm that is off by 2^-22."""
+    query = steered_queries(2, 7, 128, torch.float16, 71)
+    many = steered_queries(320, 32, 128, torch.float16, 73)
+    for small in (0.0, 2.0 ** -17, 1.0, 2.0 ** 12):
+        for q, lens, kv_heads in ((query, [150, 2000], 1), (many, [320], 16)):
+            cache = steered_cache(lens, {}, kv_heads, 128, 16, small, 70)
+            _, lse = q4_cache.attention(q, *cache, return_lse=True)
+            _, want, _, bound = q4_oracle.attention(q, *cache)
+            assert ((lse.double().cpu() - want).abs() <= bound).all()
