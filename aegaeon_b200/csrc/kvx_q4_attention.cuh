@@ -72,7 +72,7 @@ struct AttnArgs {
   int q_vec, o_vec;         // 16-byte accesses serve for query, 8-byte ones for out
   int o_vec16;              // 16-byte ones for out
   float* part_o;            // [2 * shares][rows][D]
-  float2* part_ml;          // [2 * shares][rows] (running maximum, sum)
+  float2* part_ml;          // [2 * shares][rows] (reference point, sum of p)
   Joint* joints;            // [shares], or [items]
   int joint_by_item;
 };
@@ -537,8 +537,8 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const Fragments<
         float y[2] = {p.x * vs[u][r], p.y * vs[u][r]};
         float z[2] = {fmaf(p.x, vz[u][r], st.z[n][0]), fmaf(p.y, vz[u][r], st.z[n][1])};
         if (kMasked) {  // a hidden token's scale and zero may be anything
-          if (p.x == 0.f) y[0] = 0.f, z[0] = st.z[n][0];
-          if (p.y == 0.f) y[1] = 0.f, z[1] = st.z[n][1];
+          if (x[u][n][2 * r] == kNegInf) y[0] = 0.f, z[0] = st.z[n][0];
+          if (x[u][n][2 * r + 1] == kNegInf) y[1] = 0.f, z[1] = st.z[n][1];
         }
         st.z[n][0] = z[0], st.z[n][1] = z[1];
         const __half2 h = __floats2half2_rn(y[0], y[1]);
@@ -1070,8 +1070,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT))
 
 // ---- the join of partial results ---------------------------------------------
 
-// Weight of a piece with (maximum, sum) ml against the maximum m of all: a piece
-// without a finite score counts for nothing, unless a NaN is in it.
+// Weight of a piece with (reference point, sum) ml against the largest of all, m: a
+// piece without a finite score counts for nothing, unless a NaN is in it.
 __device__ __forceinline__ float piece_weight(float2 ml, float m) {
   return ml.x == kNegInf ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - m);
 }
@@ -1079,7 +1079,7 @@ __device__ __forceinline__ float piece_weight(float2 ml, float m) {
 // Sums the pieces of 1 << kLg rows of a joint that fall to warp `part` of `parts`.  What
 // bounds it is the latency of its loads, so a warp has 16 (D = 256: 8) of them in
 // flight: slot q is row q & kMask of the piece q >> kLg further on.  Lane q has the
-// row's maximum and sum.
+// row's reference point and sum.
 template <int D, int kLg>
 __device__ __forceinline__ void join_pieces(const AttnArgs& a, const Joint& x, int kRows, int r0,
                                             int rows, int part, int parts, float& m, float& l,
@@ -1113,14 +1113,15 @@ __device__ __forceinline__ void join_pieces(const AttnArgs& a, const Joint& x, i
                       : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     const float f = piece_weight(ml, m);
-    float add = f != 0.f ? f * ml.y : 0.f;
+    float add = f * ml.y;
 #pragma unroll
     for (int d = 1 << kLg; d < kSlots; d *= 2) add += __shfl_xor_sync(~0u, add, d);
     l += add;
 #pragma unroll
     for (int q = 0; q < kSlots; ++q) {
       const float fq = __shfl_sync(~0u, f, q);
-      if (fq != 0.f) {  // what a piece without weight holds may be anything
+      // Whatever the weight, which may have underflowed: a piece's NaN is the row's.
+      if (k0 + (q >> kLg) < count) {
 #pragma unroll
         for (int i = 0; i < kParts; ++i) {
           float4& s = o[q & kMask][i];

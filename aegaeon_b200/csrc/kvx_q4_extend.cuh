@@ -641,8 +641,8 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
             float2 w = mul2(p, k ? make_float2(sc.z, sc.w) : make_float2(sc.x, sc.y));
             float2 zn = fma2(p, k ? make_float2(zc.z, zc.w) : make_float2(zc.x, zc.y), z);
             if (!plain) {  // a hidden token's scale and zero may be anything
-              if (p.x == 0.f) w.x = 0.f, zn.x = z.x;
-              if (p.y == 0.f) w.y = 0.f, zn.y = z.y;
+              if (y[c + k] == kNegInf) w.x = 0.f, zn.x = z.x;
+              if (y[c + k + 1] == kNegInf) w.y = 0.f, zn.y = z.y;
             }
             z = zn;
             const __half2 half = __floats2half2_rn(w.x, w.y);

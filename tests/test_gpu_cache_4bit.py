@@ -245,3 +245,45 @@ def test_log_sum_exp_with_any_value_scale():
             _, lse = q4_cache.attention(q, *cache, return_lse=True)
             _, want, _, bound = q4_oracle.attention(q, *cache)
             assert ((lse.double().cpu() - want).abs() <= bound).all()
+
+
+# ---- rows marked as NaN ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("push", [0.0, 60.0])
+@pytest.mark.parametrize("token", [3, 70, 145, 2500])
+def test_a_nan_value_reaches_every_row_that_sees_it(token, push):
+    """Even where the weight underflows (push 60: a weight of 2^-245): its product with a
+    NaN is none the less a NaN, in masked tiles, in plain ones and in joined pieces."""
+    bad = torch.full((128,), math.nan, device="cuda")
+    n = 150 if token < 150 else 4000
+    cache = steered_cache([n, 30], {(0, token): (push, bad)}, 1, 128, 16, 1.0, 80)
+    q = steered_queries(8, 7, 128, torch.bfloat16, 81)  # positions n - 4 ... n - 1
+    got = q4_cache.attention(q, *cache)
+    sees = torch.arange(n - 4, n) >= token
+    assert torch.equal(got[:4].isnan().all(-1).all(-1).cpu(), sees)
+    assert torch.equal(got[:4].isnan().any(-1).any(-1).cpu(), sees)
+    assert torch.isfinite(got[4:]).all()
+
+
+@pytest.mark.parametrize("push", [0.0, 60.0])
+def test_a_nan_value_among_many_rows(push):
+    bad = torch.full((128,), math.nan, device="cuda")
+    for token in (0, 131, 300):
+        cache = steered_cache([340], {(0, token): (push, bad)}, 16, 128, 16, 1.0, 90)
+        got = q4_cache.attention(steered_queries(340, 32, 128, torch.float16, 91), *cache)
+        assert torch.isfinite(got[:token]).all()
+        assert got[token:].isnan().all()
+        got = q4_cache.attention(steered_queries(340, 32, 128, torch.float16, 92), *cache, window=40)
+        assert got[token:token + 40].isnan().all()
+        assert torch.isfinite(got[:token]).all() and torch.isfinite(got[token + 40:]).all()
+
+
+def test_a_nan_value_in_a_stretch_without_weight():
+    """Whole pieces of a long sequence whose weights underflow against the others'."""
+    zero, bad = torch.zeros(128, device="cuda"), torch.full((128,), math.nan, device="cuda")
+    stretch = {(0, t): (60.0, zero) for t in range(900, 1500)}
+    q = steered_queries(1, 7, 128, torch.bfloat16, 95)
+    hold(q, *steered_cache([4000], stretch, 1, 128, 16, 1.0, 96))
+    stretch[0, 1200] = (60.0, bad)
+    assert q4_cache.attention(q, *steered_cache([4000], stretch, 1, 128, 16, 1.0, 96)).isnan().all()
