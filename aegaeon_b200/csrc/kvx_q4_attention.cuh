@@ -149,6 +149,9 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int n) {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr uint32_t kEven = 0x000f000fu;  // nibbles 0 and 4: code * 2^-24 in each half
 constexpr uint32_t kOdd = 0x00f000f0u;   // nibbles 1 and 5: code * 2^-20
+// Scores stay in the even codes' unit, 2^-24, until the exponent takes them: as part of a
+// row's factor, 2^24 would overflow for queries of 2^118 and more.
+constexpr float kCodeUnit = 16777216.f;
 
 template <int D>
 struct Shape {
@@ -172,8 +175,8 @@ __device__ __forceinline__ int key_dim(int j, int w) {
 // What a thread keeps of the tile's rows (its columns 2j, 2j + 1 of each eight).
 template <int NT>
 struct Columns {
-  float2 factor[NT];  // on the raw score: |scale| * log2(e) and the powers of two taken out
-  float2 sum[NT];     // sum(q), in the raw score's unit
+  float2 factor[NT];  // on the raw score: |scale| * log2(e) and the row's power of two taken out
+  float2 sum[NT];     // sum(q) times that, as the raw score counts: in 1 / kCodeUnit
   int pos[NT][2];     // position in the sequence, -1 for rows that are none
 };
 
@@ -192,9 +195,20 @@ struct Fragments {
   }
 };
 
-// A tile's query rows.  A row is scaled by a power of two so that its largest
-// element lies in [2^14, 2^15): every 16-bit float within 2^-28 of it stays
-// exact in fp16, whatever the row's range.
+// A power of two, 2^-113 to 2^127, that brings the largest element of a query row, `top`,
+// into [2^14, 2^15), and rows below 2^-113 as near to it as fp32 has a number: every 16-bit
+// float within 2^-28 of the largest stays exact in fp16.
+__device__ __forceinline__ float row_scale(float top) {
+  const int e = min(max(int(__float_as_uint(top) >> 23), 14), 254);
+  return top > 0.f ? __uint_as_float(uint32_t(127 + 14 + 127 - e) << 23) : 1.f;
+}
+// What brings that row's scores back, with the softmax scale.  Never 0, so that hidden
+// scores are -inf, and finite.
+__device__ __forceinline__ float row_factor(float scale_log2, float up) {
+  return fminf(fmaxf(scale_log2 / up, 1e-37f), 3.402823466e38f);
+}
+
+// A tile's query rows, scaled.
 template <typename T, int D, int NT>
 __device__ __forceinline__ void load_queries(const AttnArgs& a, const Seq& s, int row0, int rows,
                                              int head, Fragments<D, NT>& f, Columns<NT>& col) {
@@ -235,11 +249,9 @@ __device__ __forceinline__ void load_queries(const AttnArgs& a, const Seq& s, in
     }
 #pragma unroll
     for (int d = 1; d < 4; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    // 2^(14 - exponent of top); bounded so that both it and its inverse are normal.
-    const int e = min(max(int(__float_as_uint(top) >> 23), 20), 250);
-    float up = top > 0.f ? __uint_as_float(uint32_t(min(127 + 14 + 127 - e, 240)) << 23) : 1.f;
-    const float factor = fmaxf(a.scale_log2 * 16777216.f / up, 1e-37f);  // never 0: hidden
-    up *= a.sign;                                                        // scores are -inf
+    float up = row_scale(top);
+    const float factor = row_factor(a.scale_log2, up);
+    up *= a.sign;
 #pragma unroll
     for (int w = 0; w < kW; ++w) {
       uint32_t b[4];
@@ -255,7 +267,7 @@ __device__ __forceinline__ void load_queries(const AttnArgs& a, const Seq& s, in
     }
 #pragma unroll
     for (int d = 1; d < 4; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
-    sum *= 5.9604644775390625e-8f;
+    sum *= factor * (1.f / kCodeUnit);
     // Row 2j is with the lanes 8j ..., row 2j + 1 four lanes on.
     col.factor[n] = make_float2(__shfl_sync(~0u, factor, 8 * j), __shfl_sync(~0u, factor, 8 * j + 4));
     col.sum[n] = make_float2(__shfl_sync(~0u, sum, 8 * j), __shfl_sync(~0u, sum, 8 * j + 4));
@@ -471,18 +483,17 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const Fragments<
       const int unit = kMasked ? number[u] : 0, t = unit * 16 + g + 8 * r;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float& y = x[u][n][2 * r + c];
-          y = fmaf(k.x, y, k.y * (c ? col.sum[n].y : col.sum[n].x));
-          if constexpr (kMasked) {
-            const int p = col.pos[n][c];
-            const bool seen = unit >= 0 && t <= p && (t > p - a.window || t < a.sinks);
-            y = seen ? y : kNegInf;
-          }
+        float2 y = fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]),
+                        mul2(both(k.x), col.factor[n]), mul2(both(k.y), col.sum[n]));
+        if constexpr (kMasked) {
+          auto seen = [&](int p) {
+            return unit >= 0 && t <= p && (t > p - a.window || t < a.sinks);
+          };
+          y.x = seen(col.pos[n][0]) ? y.x : kNegInf;
+          y.y = seen(col.pos[n][1]) ? y.y : kNegInf;
         }
-        size[n][r] = fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]), col.factor[n],
-                          both(scale));
+        x[u][n][2 * r] = y.x, x[u][n][2 * r + 1] = y.y;
+        size[n][r] = fma2(y, both(kCodeUnit), both(scale));
       }
     }
 #pragma unroll
@@ -531,7 +542,8 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const Fragments<
     for (int r = 0; r < 2; ++r) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float2 p = fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]), col.factor[n], st.m[n]);
+        float2 p =
+            fma2(make_float2(x[u][n][2 * r], x[u][n][2 * r + 1]), both(kCodeUnit), st.m[n]);
         p.x = ex2(p.x), p.y = ex2(p.y);
         st.l[n] = add2(st.l[n], p);
         float y[2] = {p.x * vs[u][r], p.y * vs[u][r]};

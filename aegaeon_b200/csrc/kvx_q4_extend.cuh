@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
     const int p_hi = s.len - s.count + (row0 + tile * kTileRows + tile_rows - 1) / a.group;
     float factor, qsum = 0.f;
     {
-      // The query row, scaled by a power of two as in load_queries(), in the order
+      // The query row, scaled as in load_queries(), in the order
       // that unpack() gives the codes.
       const T* from = static_cast<const T*>(a.query) +
                       (real ? int64_t(s.start + query) * a.q_token +
@@ -504,9 +504,8 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(to_float(x[k])));
       }
-      const int e = min(max(int(__float_as_uint(top) >> 23), 20), 250);
-      float up = top > 0.f ? __uint_as_float(uint32_t(min(127 + 14 + 127 - e, 240)) << 23) : 1.f;
-      factor = fmaxf(a.scale_log2 / up, 1e-37f);  // never 0: hidden scores are -inf
+      float up = row_scale(top);
+      factor = row_factor(a.scale_log2, up);
       up *= a.sign;
 #pragma unroll 4
       for (int i = 0; i < D / 8; ++i) {

@@ -287,3 +287,20 @@ def test_a_nan_value_in_a_stretch_without_weight():
     hold(q, *steered_cache([4000], stretch, 1, 128, 16, 1.0, 96))
     stretch[0, 1200] = (60.0, bad)
     assert q4_cache.attention(q, *steered_cache([4000], stretch, 1, 128, 16, 1.0, 96)).isnan().all()
+
+
+# ---- queries of any size --------------------------------------------------------------
+
+
+@pytest.mark.parametrize("size,scale", [(5e37, 2e-38), (1e36, 1e-36), (1e-38, 1e37), (1e-37, 2e36)])
+def test_queries_at_the_ends_of_bf16(size, scale):
+    """With a softmax scale that brings the scores back, the definition is finite."""
+    for q, lens, kv_heads in ((randn((2, 7, 128), torch.float32, 101), [150, 700], 1),
+                              (randn((8, 4, 256), torch.float32, 102), [50, 90], 2),
+                              (randn((340, 32, 128), torch.float32, 103), [340], 16)):
+        q = (q.clamp(-5, 5) * size).to(torch.bfloat16)
+        cache = steered_cache(lens, {}, kv_heads, q.shape[2], 16, 0.25, 100)
+        got, lse = q4_cache.attention(q, *cache, scale=scale, return_lse=True)
+        out, want, out_bound, lse_bound = q4_oracle.attention(q, *cache, scale=scale)
+        assert ((got.double().cpu() - out).abs() <= out_bound).all()
+        assert ((lse.double().cpu() - want).abs() <= lse_bound).all()
