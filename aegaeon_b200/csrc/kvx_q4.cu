@@ -345,7 +345,9 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   a.queries = int(queries);
   a.num_tokens = int(num_tokens);
   a.group = int(group);
-  a.scale_log2 = float(std::fabs(scale) * 1.4426950408889634);
+  const double scale_log2 = std::fabs(scale) * 1.4426950408889634;
+  a.scale_log2 = float(std::min(scale_log2, 3.4e38));
+  a.scale_part = float(std::frexp(scale_log2, &a.scale_exp));
   a.sign = scale < 0 ? -1.f : 1.f;
   a.window = window == 0 || window > kNoWindow ? kNoWindow : int(window);
   a.sinks = a.window == kNoWindow ? 0 : int(std::min<int64_t>(sinks, kNoWindow));

@@ -64,6 +64,8 @@ struct AttnArgs {
   int num_tokens;
   int group;                // query heads of a kv head
   float scale_log2;         // |softmax scale| * log2(e)
+  float scale_part;         // that, as a number in [1/2, 1) (or 0)
+  int scale_exp;            // and a power of two
   float sign;               // of the softmax scale
   int window;               // kNoWindow: none
   int sinks;                // 0 without a window
@@ -202,8 +204,7 @@ __device__ __forceinline__ float row_scale(float top) {
   const int e = min(max(int(__float_as_uint(top) >> 23), 14), 254);
   return top > 0.f ? __uint_as_float(uint32_t(127 + 14 + 127 - e) << 23) : 1.f;
 }
-// What brings that row's scores back, with the softmax scale.  Never 0, so that hidden
-// scores are -inf, and finite.
+// What brings that row's scores back, with the softmax scale: above 0 and finite.
 __device__ __forceinline__ float row_factor(float scale_log2, float up) {
   return fminf(fmaxf(scale_log2 / up, 1e-37f), 3.402823466e38f);
 }
@@ -286,6 +287,10 @@ __device__ __forceinline__ float size_of(float scale) {
 // Where the reference point is put above or below the largest product, in powers of
 // two, and how far above it a product may come: below 2^14.1 in all, inside fp16.
 constexpr float kLift = 6.f, kSlack = 8.f;
+// From this size on the roundings of a score (0.25 and more, in powers of two) eat that
+// slack up.  Such a row's reference point is its largest score itself, of which every p is
+// exactly what fp32 says, 1 at most; kFar, as a limit, says so: it is looked at in each step.
+constexpr float kFarScore = 4194304.f, kFar = -3.402823466e38f;
 
 // One warp's state over the units that it takes.
 template <int D, int NT>
@@ -518,7 +523,24 @@ __device__ __forceinline__ void attend_units(const AttnArgs& a, const Fragments<
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
         by[c] = 1.f;
-        if (t != kNegInf) {
+        const bool far = limit == kFar || (t != kNegInf && fabsf(t) >= kFarScore);
+        if (__any_sync(~0u, far)) {
+          float y = kNegInf;
+#pragma unroll
+          for (int u = 0; u < kAb; ++u) y = max3(y, x[u][n][c], x[u][n][2 + c]);
+          y *= kCodeUnit;
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) y = fmaxf(y, __shfl_xor_sync(~0u, y, d));
+          if (far) {
+            if (limit != kNegInf) {
+              y = fmaxf(y, -m);
+              by[c] = ex2(-y - m);
+            }
+            m = -y;
+            limit = kFar;
+          }
+        }
+        if (!far && t != kNegInf) {
           t = ceilf(t);
           if (limit != kNegInf) by[c] = ex2(kLift - t - m);
           m = kLift - t;

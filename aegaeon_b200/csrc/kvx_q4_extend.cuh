@@ -44,7 +44,7 @@ struct ExtendShape {
 };
 
 struct ExtendShared {
-  float ks[2][kExtendTokens], kz[2][kExtendTokens];  // K: scale, zero + 8 scale
+  float ks[2][kExtendTokens], kz[2][kExtendTokens];  // K: scale, zero + 8 scale, by scale_part
   float vs[2][kExtendTokens], vz[2][kExtendTokens];  // V
   float top[2][4];                           // largest V scale, by warp
   int number[2][kExtendTokens / 16];         // the block's units, -1: not there
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
             value.there && token <= v.p_hi && (token > v.p_lo - a.window || token < a.sinks);
         const float2 kp = seen ? half2_at(value.param[0]) : make_float2(0.f, 0.f);
         const float2 vp = seen ? half2_at(value.param[1]) : make_float2(0.f, 0.f);
-        sh.ks[st][t] = kp.x, sh.kz[st][t] = fmaf(8.f, kp.x, kp.y);
+        sh.ks[st][t] = kp.x * a.scale_part, sh.kz[st][t] = fmaf(8.f, kp.x, kp.y) * a.scale_part;
         sh.vs[st][t] = vp.x, sh.vz[st][t] = fmaf(8.f, vp.x, vp.y);
         if (t % 16 == 0) sh.number[st][t / 16] = value.there ? n : -1;
         float top = fabsf(vp.x);
@@ -505,7 +505,9 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(to_float(x[k])));
       }
       float up = row_scale(top);
-      factor = row_factor(a.scale_log2, up);
+      // The power of two of the softmax scale; the rest of it is in ks and kz.
+      const int k = a.scale_exp + 127 - int(__float_as_uint(up) >> 23);
+      factor = __uint_as_float(uint32_t(min(max(k, -126), 127) + 127) << 23);
       up *= a.sign;
 #pragma unroll 4
       for (int i = 0; i < D / 8; ++i) {
@@ -591,10 +593,19 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
           if (__any_sync(~0u, top + minus_r > limit)) {
             float f = 1.f;
             if (top + minus_r > limit) {
-              const float to = kLift - ceilf(top);
-              if (limit != kNegInf) f = ex2(to - minus_r);
+              float to = kLift - ceilf(top);
+              if (limit == kFar || fabsf(top) >= kFarScore) {
+                top = kNegInf;
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) top = max3(top, y[c], y[c + 1]);
+                to = -ceilf(top * factor);
+                if (limit != kNegInf) to = fminf(to, minus_r), f = ex2(to - minus_r);
+                limit = kFar;
+              } else {
+                if (limit != kNegInf) f = ex2(to - minus_r);
+                limit = kLift + kSlack;
+              }
               minus_r = to;
-              limit = kLift + kSlack;
             }
             l.x *= f, l.y *= f, z.x *= f, z.y *= f;
             if (i > 0) {  // the scores waited for the last block's outputs

@@ -304,3 +304,40 @@ def test_queries_at_the_ends_of_bf16(size, scale):
         out, want, out_bound, lse_bound = q4_oracle.attention(q, *cache, scale=scale)
         assert ((got.double().cpu() - out).abs() <= out_bound).all()
         assert ((lse.double().cpu() - want).abs() <= lse_bound).all()
+
+
+@pytest.mark.parametrize("size,small", [
+    (3e5, 1.0), (1e6, 2.0 ** -17), (1e7, 1.0), (1e8, 2.0 ** -17), (1e9, 2.0 ** 12), (1e37, 1.0),
+    (1e37, 2.0 ** -14)])
+def test_scores_as_large_as_fp32_holds(size, small):
+    """Where fp32 counts scores in whole numbers and more, the largest takes all.  Keys of
+    codes 0 and 15 alone."""
+    n, dim = 320, 128
+    for tokens, heads, kv_heads in ((1, 7, 1), (320, 32, 16)):
+        kp, vp, tables, lens = steered_cache([n], {}, kv_heads, dim, 16, small, 110)
+        g = torch.Generator(device="cuda").manual_seed(112)
+        key = torch.randint(0, 2, (n, kv_heads, dim), generator=g, device="cuda").float()
+        key[..., 0], key[..., 1] = 0.0, 1.0
+        j = torch.arange(n, device="cuda")
+        slots = tables[0].long()[j // 16] * 16 + j % 16
+        _, value = q4_cache.read(kp, vp, slots, head_dim=dim, dtype=torch.float32)
+        q4_cache.write(key, value, kp, vp, slots)
+        q = (randn((tokens, heads, dim), torch.float32, 111).clamp(-3, 3) * size).to(torch.bfloat16)
+        got, lse = q4_cache.attention(q, kp, vp, tables, lens, return_lse=True)
+        key, value = (t.double().repeat_interleave(heads // kv_heads, 1) for t in
+                      q4_cache.read(kp, vp, slots, head_dim=dim, dtype=torch.float32))
+        score = torch.einsum("thd,jhd->thj", q.double(), key) / math.sqrt(dim)
+        place = torch.arange(n - tokens, n, device="cuda")
+        score.masked_fill_((torch.arange(n, device="cuda") > place[:, None])[:, None], -math.inf)
+        two = score.topk(2, -1).values
+        # by how much a score is off: (dim/16 + 4) 2^-23 of the sum of |q| |k|
+        off = torch.einsum("thd,jhd->thj", q.double().abs(), key.abs()).amax(-1) / math.sqrt(dim)
+        off *= (dim / 16 + 4) * 2.0 ** -23
+        clear = two[..., 0] - two[..., 1] > 4 * off + 40  # others weigh e^-40 at most
+        assert clear[1 if tokens > 1 else 0:].double().mean() > 0.8
+        want = value[score.argmax(-1), torch.arange(heads, device="cuda")]
+        # half a step of bf16; fp16's half step 2^-25 in the weight of a code, 8 from the middle
+        bound = 2.0 ** -8 * want.abs() + 8 * 2.0 ** -25 + 8 * 2.0 ** -11 * small
+        assert torch.isfinite(got).all()
+        assert ((got.double() - want).abs() <= bound)[clear].all()
+        assert ((lse.double() - two[..., 0]).abs() <= off + 6 + 2.0 ** -22 * two[..., 0].abs()).all()
