@@ -14,12 +14,12 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -110,10 +110,110 @@ int check_rows(const at::Tensor& key, const at::Tensor& value, int64_t tokens,
   return kind;
 }
 
-// Whether two tensors share bytes, as far as their strides tell.
-bool overlap(const at::Tensor& x, const at::Tensor& y) {
-  const at::MemOverlapStatus s = at::get_overlap_status(x, y);
-  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
+// The bytes of a tensor: runs of `run` bytes at base + sums of multiples of the strides,
+// largest stride first.  Neighbouring dimensions that lie like one are one.
+struct Extent {
+  static constexpr int kMost = 8;
+  const char* base = nullptr;
+  int64_t run = 0, span = 0;  // of one run; from the first byte to behind the last
+  int dims = 0;
+  int64_t size[kMost], stride[kMost];
+  bool known = true;  // false: more dimensions than this can hold
+
+  explicit Extent(const at::Tensor& t) {
+    if (t.numel() == 0) return;
+    base = static_cast<const char*>(t.const_data_ptr());
+    run = t.element_size();
+    std::pair<int64_t, int64_t> d[16];  // (stride, size)
+    int n = 0;
+    if (t.dim() > 16) known = false;
+    for (int64_t i = 0; known && i < t.dim(); ++i)
+      if (t.size(i) > 1) d[n++] = {t.stride(i) * t.element_size(), t.size(i)};
+    std::sort(d, d + n);
+    for (int i = 0; i < n; ++i) {
+      if (dims == 0 && d[i].first == run) {
+        run *= d[i].second;
+      } else if (dims > 0 && d[i].first == stride[dims - 1] * size[dims - 1]) {
+        size[dims - 1] *= d[i].second;
+      } else if (dims == kMost) {
+        known = false;
+      } else {
+        stride[dims] = d[i].first, size[dims] = d[i].second;
+        ++dims;
+      }
+    }
+    std::reverse(stride, stride + dims);
+    std::reverse(size, size + dims);
+    span = span_from(0);
+  }
+  int64_t span_from(int d) const {
+    int64_t n = run;
+    for (; d < dims; ++d) n += (size[d] - 1) * stride[d];
+    return n;
+  }
+  // Whether no byte is in two of its runs, which is so where each stride passes
+  // all that lies inside it.
+  bool apart() const {
+    for (int d = 0; d < dims; ++d)
+      if (stride[d] < span_from(d + 1)) return false;
+    return known;
+  }
+};
+
+// Whether x from dimension dx on, at 0, and y from dy on, at `at`, share a byte.  Takes
+// the larger of the two outermost strides (both at once where they are one) and
+// follows those steps alone that bring the spans together.  After `left` steps the answer
+// is yes: refusing such strides is better than racing.
+bool meet(const Extent& x, int dx, const Extent& y, int dy, int64_t at, int* left) {
+  const int64_t nx = x.span_from(dx), ny = y.span_from(dy);
+  if (at >= nx || -at >= ny) return false;
+  if ((dx == x.dims && dy == y.dims) || --*left < 0) return true;
+  const int64_t sx = dx < x.dims ? x.stride[dx] : 0, sy = dy < y.dims ? y.stride[dy] : 0;
+  const int64_t s = std::max(sx, sy);
+  if (s == 0) return true;  // outermost dimensions that do not move
+  const int ix = dx + (sx == s), iy = dy + (sy == s);
+  // at + k s, k from -(steps of x) to the steps of y
+  const int64_t low = sx == s ? -(x.size[dx] - 1) : 0, high = sy == s ? y.size[dy] - 1 : 0;
+  const int64_t mx = x.span_from(ix), my = y.span_from(iy);
+  // the steps with -my < at + k s < mx
+  auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+  const int64_t first = std::max(low, floor_div(-my - at, s) + 1);
+  const int64_t last = std::min(high, -floor_div(at - mx, s) - 1);
+  for (int64_t k = first; k <= last; ++k) {
+    if (meet(x, ix, y, iy, at + k * s, left)) return true;
+    if (*left < 0) return true;
+  }
+  return false;
+}
+
+// First byte of a tensor and the one behind its last.
+std::pair<const char*, const char*> range(const at::Tensor& t) {
+  const char* base = static_cast<const char*>(t.const_data_ptr());
+  if (t.numel() == 0) return {base, base};
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {base, base + (last + 1) * t.element_size()};
+}
+
+// Whether two tensors share bytes (yes, too, where their strides make it too long to tell).
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const auto ra = range(a), rb = range(b);  // of most pairs they tell: 20 ns
+  if (ra.first == ra.second || rb.first == rb.second || ra.second <= rb.first ||
+      rb.second <= ra.first)
+    return false;
+  const Extent x(a), y(b);
+  if (!x.known || !y.known) return true;
+  int left = 10000;
+  return meet(x, 0, y, 0, y.base - x.base, &left);
+}
+
+// An output must have one place for each element and share none with the inputs.
+void check_output(const at::Tensor& t, const char* name,
+                  std::initializer_list<std::pair<const at::Tensor*, const char*>> others) {
+  REQUIRE(t.is_non_overlapping_and_dense() || Extent(t).apart(),
+          std::string("the elements of ") + name + " overlap one another");
+  for (const auto& [other, what] : others)
+    REQUIRE(!overlap(t, *other), std::string(name) + " must not overlap " + what);
 }
 
 int64_t check_slots(const at::Tensor& s, c10::Device device) {
@@ -200,8 +300,13 @@ PyObject* py_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                key.size(2));
   const int64_t tokens = check_slots(slots, c.device);
   const int kind = check_rows(key, value, tokens, c);
-  REQUIRE(!overlap(THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3])),
-          "key and value pages to write to must not overlap");
+  const at::Tensor &key_pages = THPVariable_Unpack(args[2]),
+                   &value_pages = THPVariable_Unpack(args[3]);
+  check_output(key_pages, "key pages to write to",
+               {{&value_pages, "the value pages"}, {&key, "key"}, {&value, "value"},
+                {&slots, "slots"}});
+  check_output(value_pages, "value pages to write to",
+               {{&key, "key"}, {&value, "value"}, {&slots, "slots"}});
   if (tokens == 0) return PyLong_FromLong(0);
   return PyLong_FromLong(on_device(c.device, [&](void* stream) {
     return g_write(key.data_ptr(), value.data_ptr(), kind, tokens, key.stride(0), key.stride(1),
@@ -232,9 +337,18 @@ PyObject* py_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   } else {
     key = tensor(args[5], "out");
     value = tensor(args[6], "out");
-    REQUIRE(!overlap(key, value), "the key and value rows of out must not overlap");
   }
   const int kind = check_rows(key, value, tokens, c);
+  if (args[5] != Py_None) {
+    const at::Tensor &key_pages = THPVariable_Unpack(args[0]),
+                     &value_pages = THPVariable_Unpack(args[1]);
+    check_output(key, "the key rows of out",
+                 {{&value, "its value rows"}, {&key_pages, "the key pages"},
+                  {&value_pages, "the value pages"}, {&slots, "slots"}});
+    check_output(value, "the value rows of out",
+                 {{&key_pages, "the key pages"}, {&value_pages, "the value pages"},
+                  {&slots, "slots"}});
+  }
   int rc = 0;
   if (tokens)
     rc = on_device(c.device, [&](void* stream) {
@@ -316,7 +430,12 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     REQUIRE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() &&
                 out.device() == c.device && out.stride(2) == 1,
             "out must have the shape, type and device of query and contiguous rows");
-    REQUIRE(!overlap(out, q), "out must not overlap query: other warps still read it");
+    // Other warps still read all of these when a first row is written.
+    check_output(out, "out",
+                 {{&q, "query"}, {&THPVariable_Unpack(args[1]), "the key pages"},
+                  {&THPVariable_Unpack(args[2]), "the value pages"}, {&tables, "block_tables"},
+                  {&lens, "seq_lens"}});
+    if (args[5] != Py_None) check_output(out, "out", {{&THPVariable_Unpack(args[5]), "query_starts"}});
   }
   const int want_lse = PyObject_IsTrue(args[10]);
   if (want_lse < 0) return nullptr;
@@ -353,6 +472,14 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_CALL
 }
 
+// overlap(a, b): whether two tensors share memory, as the checks above see it
+PyObject* py_overlap(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!count(n, 2, "overlap")) return nullptr;
+  BEGIN_CALL
+  return PyBool_FromLong(overlap(tensor(args[0], "a"), tensor(args[1], "b")));
+  END_CALL
+}
+
 #define METHOD(name, doc) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_##name)), \
    METH_FASTCALL, doc}
@@ -360,6 +487,7 @@ PyMethodDef kMethods[] = {
     METHOD(bind, "bind(write, read, attention, attention_workspace)"),
     METHOD(write, "kvx_q4_write on tensors; returns the status"),
     METHOD(read, "kvx_q4_read on tensors; returns (status, key, value)"),
+    METHOD(overlap, "overlap(a, b): whether two tensors share memory"),
     METHOD(attention, "kvx_q4_attention on tensors; returns (status, out, lse)"),
     {nullptr, nullptr, 0, nullptr}};
 

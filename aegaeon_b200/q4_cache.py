@@ -20,7 +20,8 @@ tensors as the segments of a ``KVSwapper``, or a view of them in a 2-byte type
 Slot ``s`` is token ``s % block_size`` of block ``s // block_size``.  Every call
 is queued on the current stream of its tensors' device and may be captured into
 a CUDA graph; nothing is read back.  What the host can see is checked before
-anything is queued (ValueError, TypeError); a slot, block id or length in device
+anything is queued (ValueError, TypeError), also that what a call writes overlaps
+neither itself nor what it reads; a slot, block id or length in device
 memory that is outside its buffer is skipped by the kernels and shows in
 ``_lib.device_status``.  None of them has a gradient: a tensor that requires one
 is refused unless gradients are off.  The reference has no counterpart (its caches hold

@@ -364,7 +364,8 @@ int kvx_safetensors_meta_json(const char* file_path, char* out,
  * All device pointers; nothing is read back: a slot, block id or length that
  * is outside its buffer is skipped by the kernels and reported by
  * kvx_device_status (KVX_ERR_BLOCK_ID, KVX_ERR_EXTENT).  Every call may be
- * captured into a CUDA graph.
+ * captured into a CUDA graph.  What a call writes must overlap neither itself
+ * nor anything that it reads.
  *
  * kvx_q4_write: quantises key and value [num_tokens][kv_heads][head_dim] into
  * slots[i] of token i (negative: the row is skipped, as padding is).  With x a
@@ -386,8 +387,7 @@ int kvx_safetensors_meta_json(const char* file_path, char* out,
  * tokens j <= p, with window > 0 only those with j > p - window or j < sinks.
  * out: softmax(scale * q k) v, lse (optional, [num_tokens][num_heads]): the
  * natural log-sum-exp of the scores.  A row that sees nothing gives 0 and
- * -inf.  Rows behind the last sequence are left as they were.  out must not
- * overlap query.  workspace:
+ * -inf.  Rows behind the last sequence are left as they were.  workspace:
  * kvx_q4_attention_workspace() bytes, 16-byte aligned, for this call alone
  * until it has finished; rows_per_sequence is the call's num_tokens (divided
  * by batch without query_starts) * num_heads / kv_heads.                       */

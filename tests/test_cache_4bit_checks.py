@@ -1,0 +1,57 @@
+"""Checks of the 4-bit cache's arguments that need no GPU."""
+
+import random
+
+import torch
+
+from aegaeon_b200 import _lib
+
+
+def places(t):
+    """The elements of the storage that a tensor names."""
+    at = torch.zeros((), dtype=torch.int64) + t.storage_offset()
+    for n, s in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(n) * s
+    return at.flatten().tolist()
+
+
+def test_overlap_of_strided_views():
+    """Any two views of one storage, against a list of their elements."""
+    overlap = _lib.q4().overlap
+    rng = random.Random(5)
+    base = torch.zeros(100000, dtype=torch.int16)
+    shared = apart = 0
+    for _ in range(4000):
+        views = []
+        for _ in range(2):
+            dims = rng.randint(1, 3)
+            size = [rng.randint(1, 5) for _ in range(dims)]
+            stride, inner = [], 1
+            for n in reversed(size):  # mostly nested, as views of one tensor are
+                stride.append(rng.choice([inner, inner + rng.randint(0, 6), rng.randint(0, 40)]))
+                inner = max(1, stride[-1] * n)
+            stride.reverse()
+            views.append(base.as_strided(size, stride, rng.randint(0, 300)))
+        want = not set(places(views[0])).isdisjoint(places(views[1]))
+        assert overlap(*views) == want, [(v.shape, v.stride(), v.storage_offset()) for v in views]
+        shared, apart = shared + want, apart + (not want)
+    assert shared > 500 and apart > 500
+
+
+def test_overlap_of_the_views_that_callers_have():
+    overlap = _lib.q4().overlap
+    qkv = torch.zeros(100, 48, 128, dtype=torch.float16)
+    q, k, v = qkv[:, :32], qkv[:, 32:40], qkv[:, 40:]
+    assert overlap(q, qkv[:, :32]) and overlap(q, qkv[:, 31:40]) and overlap(qkv, v)
+    assert not overlap(q, k) and not overlap(k, v) and not overlap(q, torch.zeros(5))
+    pages = torch.zeros(50, 4, 2, 8, 1088, dtype=torch.uint8)  # blocks, layers, K and V
+    for i in range(4):
+        for j in range(4):
+            for a in range(2):
+                for b in range(2):
+                    assert overlap(pages[:, i, a], pages[:, j, b]) == ((i, a) == (j, b))
+    assert overlap(pages[:, 1], pages[7]) and not overlap(pages[:7], pages[7:])
+    empty = qkv[:0]
+    assert not overlap(empty, qkv) and not overlap(qkv, empty)
+    long = torch.zeros(1, dtype=torch.float16).expand(100000, 7, 128)  # one element, many names
+    assert overlap(long, long) and not overlap(long, qkv)

@@ -341,3 +341,66 @@ def test_scores_as_large_as_fp32_holds(size, small):
         assert torch.isfinite(got).all()
         assert ((got.double() - want).abs() <= bound)[clear].all()
         assert ((lse.double() - two[..., 0]).abs() <= off + 6 + 2.0 ** -22 * two[..., 0].abs()).all()
+
+
+# ---- arguments that share memory -------------------------------------------------------
+
+
+def test_outputs_that_share_memory_with_inputs_are_refused():
+    block, dim = 16, 128
+    kp, vp, tables, lens = steered_cache([40, 20], {}, 2, dim, block, 1.0, 120)
+    qkv = randn((2, 8, dim), torch.bfloat16, 121)
+    att = lambda q, out: q4_cache.attention(q, kp, vp, tables, lens, out=out)  # noqa: E731
+    want = q4_cache.attention(qkv[:, :4].clone(), kp, vp, tables, lens)
+    before = qkv.clone()
+    for out in (qkv[:, :4], qkv[:, 1:5], qkv[:, 3:7]):
+        with pytest.raises(ValueError, match="overlap"):
+            att(qkv[:, :4], out)
+    with pytest.raises(ValueError, match="overlap"):  # every row in one place
+        att(qkv[:, :4], torch.empty((1, 4, dim), dtype=torch.bfloat16, device="cuda").expand(2, 4, dim))
+    with pytest.raises(ValueError, match="overlap"):  # in the pages
+        att(qkv[:, :4], kp.view(-1)[:2 * 4 * dim * 2].view(torch.bfloat16).view(2, 4, dim))
+    numbers = torch.zeros(2 * 4 * dim, dtype=torch.int32, device="cuda")
+    numbers[:2] = lens
+    with pytest.raises(ValueError, match="overlap"):  # in the lengths
+        q4_cache.attention(qkv[:, :4], kp, vp, tables, numbers[:2],
+                           out=numbers.view(torch.bfloat16)[:2 * 4 * dim].view(2, 4, dim))
+    assert torch.equal(qkv, before)
+    assert torch.equal(att(qkv[:, :4], qkv[:, 4:]), want)  # beside the queries: allowed
+    assert torch.equal(qkv[:, :4], before[:, :4]) and torch.equal(qkv[:, 4:], want)
+
+    slots = torch.arange(3, device="cuda")
+    rows = torch.zeros((3, 5, dim), dtype=torch.bfloat16, device="cuda")
+    read = lambda a, b: q4_cache.read(kp, vp, slots, head_dim=dim, out=(a, b))  # noqa: E731
+    for a, b in ((rows[:, :2], rows[:, 1:3]), (rows[:, 2:4], rows[:, 2:4]),
+                 (rows[:1, :2].expand(3, 2, dim), rows[:, 2:4]),
+                 (rows[:, :2], vp.view(-1)[:3 * 2 * dim * 2].view(torch.bfloat16).view(3, 2, dim))):
+        with pytest.raises(ValueError, match="overlap"):
+            read(a, b)
+    plain = q4_cache.read(kp, vp, slots, head_dim=dim)
+    got = read(rows[:, :2], rows[:, 2:4])
+    assert torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1]) and not rows[:, 4].any()
+
+    before = kp.clone()
+    with pytest.raises(ValueError, match="overlap"):
+        q4_cache.write(rows[:, :2], rows[:, 2:4], kp, kp[:], slots)
+    inside = kp.view(-1)[:3 * 2 * dim * 2].view(torch.bfloat16).view(3, 2, dim)
+    with pytest.raises(ValueError, match="overlap"):  # rows in the pages that are written
+        q4_cache.write(inside, rows[:, :2], kp, vp, slots)
+    with pytest.raises(ValueError, match="overlap"):
+        q4_cache.write(rows[:, :2], rows[:, 2:4], kp, vp, kp.view(-1)[:24].view(torch.int64))
+    assert torch.equal(kp, before)
+
+
+def test_interleaved_caches_are_written_and_read():
+    """Layers, keys and values side by side in one buffer, blocks outermost."""
+    blocks, layers, block, heads, dim = 7, 3, 16, 2, 64
+    buffer = torch.zeros((blocks, layers, 2, heads, q4_cache.head_bytes(block, dim)),
+                         dtype=torch.uint8, device="cuda")
+    slots = torch.randperm(blocks * block, device="cuda")[:50]
+    for i in range(layers):
+        key, value = randn((50, heads, dim), torch.float16, 130 + i), randn((50, heads, dim), torch.float16, 140 + i)
+        q4_cache.write(key, value, buffer[:, i, 0], buffer[:, i, 1], slots)
+        alone = q4_cache.allocate(blocks, block, heads, dim)
+        q4_cache.write(key, value, *alone, slots)
+        assert torch.equal(alone[0], buffer[:, i, 0]) and torch.equal(alone[1], buffer[:, i, 1])
