@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -57,6 +58,9 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
   if (t.requires_grad() && c10::GradMode::is_enabled())
     throw Refused{PyExc_RuntimeError, std::string(name) + " requires a gradient: the 4-bit "
                                       "cache's operators have none (detach it, or use no_grad)"};
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    throw Refused{PyExc_RuntimeError, std::string(name) + " carries a forward-mode gradient: the "
+                                      "4-bit cache's operators have none"};
   return t;
 }
 

@@ -23,8 +23,8 @@ a CUDA graph; nothing is read back.  What the host can see is checked before
 anything is queued (ValueError, TypeError), also that what a call writes overlaps
 neither itself nor what it reads; a slot, block id or length in device
 memory that is outside its buffer is skipped by the kernels and shows in
-``_lib.device_status``.  None of them has a gradient: a tensor that requires one
-is refused unless gradients are off.  The reference has no counterpart (its caches hold
+``_lib.device_status``.  None of them has a gradient: a tensor that requires one,
+or carries a forward-mode one, is refused unless gradients are off.  The reference has no counterpart (its caches hold
 16-bit values).
 """
 

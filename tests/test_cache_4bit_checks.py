@@ -2,9 +2,11 @@
 
 import random
 
+import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
-from aegaeon_b200 import _lib
+from aegaeon_b200 import _lib, q4_cache
 
 
 def places(t):
@@ -55,3 +57,23 @@ def test_overlap_of_the_views_that_callers_have():
     assert not overlap(empty, qkv) and not overlap(qkv, empty)
     long = torch.zeros(1, dtype=torch.float16).expand(100000, 7, 128)  # one element, many names
     assert overlap(long, long) and not overlap(long, qkv)
+
+
+def test_forward_mode_gradients_are_refused():
+    """A dual tensor's tangent would be lost without a word."""
+    kp, vp = q4_cache.allocate(2, 16, 2, 128, device="cpu")
+    x, slots = torch.zeros(3, 2, 128), torch.arange(3)
+    half, tables, lens = x.half(), torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    with forward_ad.dual_level():
+        dual, dual_half = forward_ad.make_dual(x, x + 1), forward_ad.make_dual(half, half + 1)
+        view = dual[:, :, :]
+        for call in (lambda: q4_cache.write(dual, x, kp, vp, slots),
+                     lambda: q4_cache.write(x, view, kp, vp, slots),
+                     lambda: q4_cache.attention(dual_half, kp, vp, tables, lens)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with torch.no_grad():  # turns reverse mode off, not this one
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                q4_cache.write(dual, x, kp, vp, slots)
+    with pytest.raises(ValueError, match="CUDA"):  # the level is over
+        q4_cache.write(dual, x, kp, vp, slots)

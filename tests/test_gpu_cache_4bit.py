@@ -8,6 +8,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import q4_oracle
 from aegaeon_b200 import _lib, q4_cache
@@ -404,3 +405,23 @@ def test_interleaved_caches_are_written_and_read():
         alone = q4_cache.allocate(blocks, block, heads, dim)
         q4_cache.write(key, value, *alone, slots)
         assert torch.equal(alone[0], buffer[:, i, 0]) and torch.equal(alone[1], buffer[:, i, 1])
+
+
+# ---- what autograd has to know ----------------------------------------------------------
+
+
+def test_forward_mode_gradients_are_refused():
+    kp, vp, tables, lens = steered_cache([20, 20], {}, 2, 128, 16, 1.0, 155)
+    slots = torch.arange(2, device="cuda")
+    rows = randn((2, 2, 128), torch.bfloat16, 156)
+    want = q4_cache.attention(rows, kp, vp, tables, lens)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(rows.clone(), rows)
+        for call in (lambda: q4_cache.attention(dual, kp, vp, tables, lens),
+                     lambda: q4_cache.attention(rows, kp, vp, tables, lens, out=dual),
+                     lambda: q4_cache.read(kp, vp, slots, head_dim=128, out=(dual, rows.clone())),
+                     lambda: q4_cache.write(rows, dual, kp, vp, slots)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        plain = forward_ad.unpack_dual(dual).primal
+        assert torch.equal(q4_cache.attention(plain, kp, vp, tables, lens), want)
