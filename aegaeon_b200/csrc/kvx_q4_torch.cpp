@@ -227,6 +227,11 @@ int64_t check_slots(const at::Tensor& s, c10::Device device) {
   return s.size(0);
 }
 
+// Tells autograd that a tensor was written to.  An inference tensor has no counter.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Runs f with the device current and its current stream.
 template <class F>
 int on_device(c10::Device device, F f) {
@@ -312,6 +317,7 @@ PyObject* py_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   check_output(value_pages, "value pages to write to",
                {{&key, "key"}, {&value, "value"}, {&slots, "slots"}});
   if (tokens == 0) return PyLong_FromLong(0);
+  written(key_pages), written(value_pages);
   return PyLong_FromLong(on_device(c.device, [&](void* stream) {
     return g_write(key.data_ptr(), value.data_ptr(), kind, tokens, key.stride(0), key.stride(1),
                    value.stride(0), value.stride(1), slots.const_data_ptr<int64_t>(), c.key,
@@ -352,6 +358,7 @@ PyObject* py_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     check_output(value, "the value rows of out",
                  {{&key_pages, "the key pages"}, {&value_pages, "the value pages"},
                   {&slots, "slots"}});
+    written(key), written(value);
   }
   int rc = 0;
   if (tokens)
@@ -439,7 +446,9 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
                  {{&q, "query"}, {&THPVariable_Unpack(args[1]), "the key pages"},
                   {&THPVariable_Unpack(args[2]), "the value pages"}, {&tables, "block_tables"},
                   {&lens, "seq_lens"}});
-    if (args[5] != Py_None) check_output(out, "out", {{&THPVariable_Unpack(args[5]), "query_starts"}});
+    if (args[5] != Py_None)
+      check_output(out, "out", {{&THPVariable_Unpack(args[5]), "query_starts"}});
+    written(out);
   }
   const int want_lse = PyObject_IsTrue(args[10]);
   if (want_lse < 0) return nullptr;

@@ -425,3 +425,44 @@ def test_forward_mode_gradients_are_refused():
                 call()
         plain = forward_ad.unpack_dual(dual).primal
         assert torch.equal(q4_cache.attention(plain, kp, vp, tables, lens), want)
+
+
+
+def test_autograd_sees_what_was_overwritten():
+    """A tensor that a gradient needs and that an operator then writes to is noticed."""
+    kp, vp, tables, lens = steered_cache([20, 20], {}, 2, 128, 16, 1.0, 150)
+    slots = torch.arange(2, device="cuda")
+    rows = randn((2, 2, 128), torch.bfloat16, 151)
+    versions = kp._version, vp._version
+    q4_cache.write(rows, rows, kp, vp, slots)
+    assert kp._version > versions[0] and vp._version > versions[1]
+    versions = kp._version, vp._version, rows._version
+    q4_cache.read(kp, vp, slots, head_dim=128)
+    q4_cache.attention(randn((2, 2, 128), torch.bfloat16, 152), kp, vp, tables, lens)
+    assert (kp._version, vp._version, rows._version) == versions
+    weight = torch.ones((2, 2, 128), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    query = randn((2, 2, 128), torch.bfloat16, 153)
+    for overwrite in (lambda t: q4_cache.attention(query, kp, vp, tables, lens, out=t),
+                      lambda t: q4_cache.read(kp, vp, slots, head_dim=128, out=(t, torch.empty_like(t))),
+                      lambda t: q4_cache.read(kp, vp, slots, head_dim=128, out=(torch.empty_like(t), t))):
+        saved = rows.clone()
+        loss = (saved * weight).sum()
+        overwrite(saved)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_inference_tensors():
+    """Pages made in inference mode are used outside it, and the other way round."""
+    slots = torch.arange(3, device="cuda")
+    rows = randn((3, 2, 128), torch.bfloat16, 160)
+    with torch.inference_mode():
+        kp, vp = q4_cache.allocate(2, 16, 2, 128)
+        q4_cache.write(rows, rows, kp, vp, slots)
+    q4_cache.write(rows, rows, kp, vp, slots)
+    a = q4_cache.read(kp, vp, slots, head_dim=128)
+    kp, vp = q4_cache.allocate(2, 16, 2, 128)
+    with torch.inference_mode():
+        q4_cache.write(rows, rows, kp, vp, slots)
+        b = q4_cache.read(kp, vp, slots, head_dim=128, out=(rows.clone(), rows.clone()))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
