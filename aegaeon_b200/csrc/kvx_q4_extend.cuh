@@ -49,10 +49,11 @@ struct ExtendShared {
   float top[2][4];                           // largest V scale, by warp
   int number[2][kExtendTokens / 16];         // the block's units, -1: not there
   // Barriers.  By stage: unpacked, read; by tile: scores there, weights there,
-  // output added; queries there.
+  // output added; queries there; all products through.
   alignas(8) uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
-  uint64_t s_full[2], p_full[2], o_full[2], q_full;
+  uint64_t s_full[2], p_full[2], o_full[2], q_full, drained;
   uint32_t tmem;
+  int cut;  // a wait has run out
   int64_t scan[kExtendThreads / 32];
   Place found;
 };
@@ -114,6 +115,13 @@ __device__ __forceinline__ void products_done(uint64_t* bar) {
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
           smem_of(bar))
       : "memory");
+}
+
+// Waits for all products, with the same limit.  Out of line: inside the kernel its few
+// instructions took 1 us of each CTA's time (pieces of 411 with a window, 64.5 instead of 63.2).
+__device__ __noinline__ void drain(uint64_t* bar) {
+  products_done(bar);
+  wait_phase(bar, 0);
 }
 
 #define KVX_OUT4(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3])
@@ -357,6 +365,8 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
         init(&sh.s_full[i], 1), init(&sh.o_full[i], 1);
       }
       init(&sh.q_full, uint32_t(4 * tiles));
+      init(&sh.drained, 1);
+      sh.cut = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
@@ -402,7 +412,7 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
           tmem_after();
           scores(1, i);
         }
-        products_done(&sh.k_free[st]);
+        if (i + 2 < blocks) products_done(&sh.k_free[st]);  // somebody waits for it
         waiter.wait(&sh.v_full[st], round);
         waiter.wait(&sh.p_full[0], i & 1);
         tmem_after();
@@ -418,7 +428,7 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
           tmem_after();
           outputs(1, i);
         }
-        products_done(&sh.v_free[st]);
+        if (i + 2 < blocks) products_done(&sh.v_free[st]);
       }
     }
     __syncwarp();
@@ -703,11 +713,20 @@ __global__ void __launch_bounds__(kExtendThreads, 1) q4_extend(const __grid_cons
       a.lse[token * (int64_t(heads) * a.group) + head_out] = log_sum(-minus_r, total);
     }
   }
-  if (!waiter.fine) atomicExch(&g_q4_status, 8 /* KVX_ERR_DEVICE_TIMEOUT */);
+  if (!waiter.fine) {
+    sh.cut = 1;
+    atomicExch(&g_q4_status, 8 /* KVX_ERR_DEVICE_TIMEOUT */);
+  }
   tmem_before();
   __syncthreads();
   if (warp == 12) {
     tmem_after();
+    // The last outputs were waited for, and with them every product.  Not so where a wait
+    // ran out: none of them may outlive the block's memory.
+    if (sh.cut && lane == 0) {
+      drain(&sh.drained);
+    }
+    __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "n"(S::kColumns));
   }

@@ -466,3 +466,23 @@ def test_inference_tensors():
         q4_cache.write(rows, rows, kp, vp, slots)
         b = q4_cache.read(kp, vp, slots, head_dim=128, out=(rows.clone(), rows.clone()))
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# ---- short caches in the kernel of many rows --------------------------------------------
+
+
+@pytest.mark.parametrize("n", [1, 16, 100, 128, 129, 256, 257, 384, 385])
+@pytest.mark.parametrize("queries", [64, 100])
+def test_many_rows_over_few_blocks(n, queries):
+    """One, two, three and four blocks of 128 tokens, for CTAs of one tile (64 queries of two
+    heads) and of two.  Calls follow one another at once: nothing of a block that has ended
+    may reach the next one."""
+    cache = steered_cache([n], {}, 148, 64, 16, 0.5, 170)
+    q = steered_queries(queries, 296, 64, torch.float16, 171)
+    results = [q4_cache.attention(q, *cache) for _ in range(6)]
+    for r in results[1:]:
+        assert torch.equal(r, results[0])
+    some = slice(0, 4)  # two kv heads hold for all
+    pages = [p[:, :2].contiguous() for p in cache[:2]]
+    want, _, bound, _ = q4_oracle.attention(q[:, some], *pages, *cache[2:])
+    assert ((results[0][:, some].double().cpu() - want).abs() <= bound).all()
