@@ -50,6 +50,8 @@ int cache_of(const void* key_pages, const void* value_pages, int64_t stride, int
                   "cache pages and the stride between them must be multiples of 16 bytes");
     if (stride < kv_heads * head_bytes)
       return fail(KVX_ERR_INVALID_ARGUMENT, "page stride below the size of a page");
+    if (stride > INT64_MAX / num_blocks)
+      return fail(KVX_ERR_INVALID_ARGUMENT, "pages beyond the address space");
   }
   out->pages[0] = static_cast<uint8_t*>(const_cast<void*>(key_pages));
   out->pages[1] = static_cast<uint8_t*>(const_cast<void*>(value_pages));
@@ -98,9 +100,11 @@ int run_rows(bool write, RowArgs& a, int dtype, int64_t num_tokens, int64_t head
   for (const Rows& r : a.rows)
     if (!aligned(r.base, element_size(dtype)))
       return fail(KVX_ERR_INVALID_ARGUMENT, "rows are not aligned to their type");
-  const int64_t num_rows = num_tokens * a.cache.kv_heads;
-  if (num_tokens > INT32_MAX || num_rows > INT32_MAX)
+  if (!aligned(a.slots, 8))
+    return fail(KVX_ERR_INVALID_ARGUMENT, "slots are not aligned to their type");
+  if (num_tokens > INT32_MAX / a.cache.kv_heads)
     return fail(KVX_ERR_INVALID_ARGUMENT, "too many tokens in one call");
+  const int64_t num_rows = num_tokens * a.cache.kv_heads;
   a.num_rows = uint32_t(num_rows);
   a.by_heads = Divisor::of(uint32_t(a.cache.kv_heads));
   a.by_block = Divisor::of(uint32_t(a.cache.block_size));
@@ -309,14 +313,16 @@ int kvx_q4_attention(const void* query, int64_t query_token_stride, int64_t quer
   if (num_tokens == 0 || batch == 0) return KVX_OK;
   if (!query || !out || !seq_lens || (!block_tables && table_width > 0))
     return fail(KVX_ERR_INVALID_ARGUMENT, "null argument");
-  if (!aligned(query, 2) || !aligned(out, 2) || !aligned(workspace, 16))
+  if (!aligned(query, 2) || !aligned(out, 2) || !aligned(workspace, 16) || !aligned(lse, 4) ||
+      !aligned(block_tables, 4) || !aligned(seq_lens, 4) || !aligned(query_starts, 4))
     return fail(KVX_ERR_INVALID_ARGUMENT, "an argument is not aligned to its type");
   const int64_t group = num_heads / kv_heads;
   if (!query_starts && num_tokens % batch)
     return fail(KVX_ERR_LENGTH_MISMATCH,
                 "without query_starts every sequence has the same number of query tokens");
-  if (num_tokens * group >= (1ll << 30) || batch >= (1ll << 30) ||
-      table_width * block_size >= (1ll << 30))
+  constexpr int64_t kMost = 1ll << 30;  // each first, so that no product passes 64 bits
+  if (num_tokens >= kMost || group >= kMost || num_tokens * group >= kMost || batch >= kMost ||
+      table_width >= kMost || table_width * block_size >= kMost)
     return fail(KVX_ERR_INVALID_ARGUMENT, "request too large for one call");
   const int64_t queries = query_starts ? num_tokens : num_tokens / batch;
   const int rows = tile_rows(queries * group, head_dim);

@@ -361,7 +361,7 @@ int kvx_safetensors_meta_json(const char* file_path, char* out,
  * in each; block_size a multiple of 16 (at most 4096); head_dim 64, 128 or 256.
  * dtype: KVX_DTYPE_*.  Strides of rows are in elements; the elements of one
  * row are contiguous.  Slot s is token s % block_size of block s / block_size.
- * All device pointers; nothing is read back: a slot, block id or length that
+ * All device pointers, aligned to their types; nothing is read back: a slot, block id or length that
  * is outside its buffer is skipped by the kernels and reported by
  * kvx_device_status (KVX_ERR_BLOCK_ID, KVX_ERR_EXTENT).  Every call may be
  * captured into a CUDA graph.  What a call writes must overlap neither itself

@@ -7,6 +7,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 from aegaeon_b200 import _lib, q4_cache
+from test_q4_refusals import P, attend, read, write
 
 
 def places(t):
@@ -77,3 +78,21 @@ def test_forward_mode_gradients_are_refused():
                 q4_cache.write(dual, x, kp, vp, slots)
     with pytest.raises(ValueError, match="CUDA"):  # the level is over
         q4_cache.write(dual, x, kp, vp, slots)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(tables=P + 2), dict(lens=P + 1), dict(starts=P + 2, tokens=3), dict(lse=P + 3),
+    dict(width=1 << 60), dict(width=(1 << 60) + 4), dict(num_heads=1 << 62, tokens=4, batch=1),
+    dict(num_heads=8 << 33), dict(tokens=1 << 62, batch=1), dict(batch=1 << 62, starts=P),
+    dict(stride=1 << 62)])
+def test_attention_refuses_what_would_wrap_or_misalign(kvx, bad):
+    """Pointers that a kernel would load 4 bytes from, and sizes whose products pass 64 bits."""
+    assert attend(kvx, **bad) == _lib.KVX_ERR_INVALID_ARGUMENT
+    assert kvx.kvx_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(slots=P + 4), dict(tokens=1 << 62), dict(tokens=1 << 31),
+                                 dict(stride=1 << 62)])
+def test_write_and_read_refuse_what_would_wrap_or_misalign(kvx, bad):
+    assert write(kvx, **bad) == _lib.KVX_ERR_INVALID_ARGUMENT
+    assert read(kvx, **bad) == _lib.KVX_ERR_INVALID_ARGUMENT
