@@ -21,11 +21,12 @@ Slot ``s`` is token ``s % block_size`` of block ``s // block_size``.  Every call
 is queued on the current stream of its tensors' device and may be captured into
 a CUDA graph; nothing is read back.  What the host can see is checked before
 anything is queued (ValueError, TypeError), also that what a call writes overlaps
-neither itself nor what it reads; a slot, block id or length in device
-memory that is outside its buffer is skipped by the kernels and shows in
-``_lib.device_status``.  None of them has a gradient: a tensor that requires one,
-or carries a forward-mode one, is refused unless gradients are off.  The reference has no counterpart (its caches hold
-16-bit values).
+neither itself nor what it reads.  What is in device memory the kernels check: a
+slot or block id outside its buffer is skipped and a length is cut to its block
+table, which shows in ``_lib.device_status``; a length below 0 counts as 0.  None
+of them has a gradient: a tensor that requires one is refused unless gradients are
+off, one that carries a forward-mode gradient always is.  What they write to counts a version
+on.  The reference has no counterpart (its caches hold 16-bit values).
 """
 
 from __future__ import annotations
@@ -82,7 +83,9 @@ def read(key_pages: torch.Tensor, value_pages: torch.Tensor, slots: torch.Tensor
          ) -> Tuple[torch.Tensor, torch.Tensor]:
     """The key and value rows of ``slots`` (int64 ``[tokens]``; negative: a row
     of zeros) as ``[tokens, kv_heads, head_dim]`` in ``dtype``, or into the
-    tensors of ``out``."""
+    tensors of ``out``.  Scale and zero are rounded, so the top of a row that reaches
+    65504 may lie above it, by less than 80: from 65520 on that is infinity in
+    float16, in an attention's output too; bfloat16 and float32 hold it."""
     key, value = (None, None) if out is None else out
     status, key, value = _lib.q4().read(key_pages, value_pages, slots, head_dim, dtype, key, value)
     if status:
@@ -103,7 +106,9 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     cache, those of this call's queries among them (``write`` them first);
     ``block_tables`` (int32 ``[batch, width]``) names their blocks.  The queries
     of a sequence are its last tokens: ``tokens / batch`` each, or rows
-    ``query_starts[b]`` to ``query_starts[b + 1]`` (int32 ``[batch + 1]``).
+    ``query_starts[b]`` to ``query_starts[b + 1]`` (int32 ``[batch + 1]``, not decreasing;
+    the call's kernel is then chosen by all its rows, so single tokens of long
+    sequences are better called apart from pieces of prompts).
     A length of 0 marks a padded sequence: its rows are 0.
 
     ``window``: a query sees itself and the ``window - 1`` tokens before it, and
@@ -111,7 +116,8 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     1 / sqrt(head_dim) by default.  ``return_lse``: also the natural
     log-sum-exp of each row's scores, float32 ``[tokens, heads]`` (-inf for a
     row that sees nothing, whose output is 0).  Rows of ``out`` behind the last
-    sequence of ``query_starts`` are left as they were."""
+    sequence of ``query_starts`` are left as they were, and the log-sum-exp has
+    nothing there."""
     status, out, lse = _lib.q4().attention(query, key_pages, value_pages, block_tables, seq_lens,
                                            query_starts, scale, window, sinks, out, return_lse)
     if status:

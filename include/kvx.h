@@ -361,11 +361,13 @@ int kvx_safetensors_meta_json(const char* file_path, char* out,
  * in each; block_size a multiple of 16 (at most 4096); head_dim 64, 128 or 256.
  * dtype: KVX_DTYPE_*.  Strides of rows are in elements; the elements of one
  * row are contiguous.  Slot s is token s % block_size of block s / block_size.
- * All device pointers, aligned to their types; nothing is read back: a slot, block id or length that
- * is outside its buffer is skipped by the kernels and reported by
- * kvx_device_status (KVX_ERR_BLOCK_ID, KVX_ERR_EXTENT).  Every call may be
- * captured into a CUDA graph.  What a call writes must overlap neither itself
- * nor anything that it reads.
+ * All device pointers, aligned to their types; nothing is read back.  What is
+ * outside its buffer is met by the kernels: slots and block ids are skipped
+ * and a length is cut to its block table, which kvx_device_status reports
+ * (KVX_ERR_BLOCK_ID, KVX_ERR_EXTENT); a length below 0 counts as 0 and starts
+ * are cut to the query, which nothing reports.  Every call may be captured
+ * into a CUDA graph.  What a call writes must overlap neither itself nor
+ * anything that it reads.
  *
  * kvx_q4_write: quantises key and value [num_tokens][kv_heads][head_dim] into
  * slots[i] of token i (negative: the row is skipped, as padding is).  With x a
@@ -376,18 +378,25 @@ int kvx_safetensors_meta_json(const char* file_path, char* out,
  * distinct; what a repeated slot holds afterwards is unspecified.
  *
  * kvx_q4_read: gives the rows of slots[i] back into key and value (rounded
- * once from 32 bits); zeros for a negative slot.
+ * once from 32 bits); zeros for a negative slot.  As scale and zero are
+ * rounded, zero + 15 scale may pass 65504 by up to 15 * 4 + 16 (their half
+ * steps; 65536 for a row from -65504 to 65504): fp16 has no number from 65520 on and gives infinity, in a row read
+ * back as in an attention's output; bf16 and fp32 hold it.
  *
  * kvx_q4_attention: causal attention of query [num_tokens][num_heads][head_dim]
  * over the cache.  Sequence b has seq_lens[b] tokens in the blocks
  * block_tables[b * table_stride + 0 ...] (table_width entries); its query
  * tokens are the last ones of them: rows [query_starts[b], query_starts[b+1])
- * of query, or num_tokens / batch each when query_starts is NULL.  Query head
+ * of query, or num_tokens / batch each when query_starts is NULL.  Starts must
+ * not decrease: rows that two sequences claim hold either's result.  Query head
  * h reads kv head h / (num_heads / kv_heads).  A query at position p sees the
  * tokens j <= p, with window > 0 only those with j > p - window or j < sinks.
  * out: softmax(scale * q k) v, lse (optional, [num_tokens][num_heads]): the
  * natural log-sum-exp of the scores.  A row that sees nothing gives 0 and
- * -inf.  Rows behind the last sequence are left as they were.  workspace:
+ * -inf.  Rows of out and lse behind the last sequence are left as they were.
+ * With query_starts a call is taken as its total: num_tokens rows decide on the
+ * kernel (many rows for enough SMs take the one that does not split a cache),
+ * so single tokens of long sequences are better called by themselves.  workspace:
  * kvx_q4_attention_workspace() bytes, 16-byte aligned, for this call alone
  * until it has finished; rows_per_sequence is the call's num_tokens (divided
  * by batch without query_starts) * num_heads / kv_heads.                       */

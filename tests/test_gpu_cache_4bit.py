@@ -486,3 +486,40 @@ def test_many_rows_over_few_blocks(n, queries):
     pages = [p[:, :2].contiguous() for p in cache[:2]]
     want, _, bound, _ = q4_oracle.attention(q[:, some], *pages, *cache[2:])
     assert ((results[0][:, some].double().cpu() - want).abs() <= bound).all()
+
+
+# ---- lengths, starts and values that the documentation speaks of -------------------------
+
+
+def test_values_beyond_fp16_when_read():
+    """Scale and zero are rounded, so a row's highest value may lie above 65504: fp16 has
+    no number for those from 65520 on and gives infinity, bfloat16 and float32 keep them."""
+    x = torch.linspace(-1, 1, 128, device="cuda")[None, None] * 65504
+    kp, vp = q4_cache.allocate(1, 16, 1, 128)
+    slots = torch.zeros(1, dtype=torch.int64, device="cuda")
+    q4_cache.write(x, x, kp, vp, slots)
+    exact = q4_oracle.values(kp, 128)[0, 0, 0]
+    assert exact.max() == 65536.0
+    for dtype in DTYPES + [torch.float32]:
+        key, _ = q4_cache.read(kp, vp, slots, head_dim=128, dtype=dtype)
+        assert torch.equal(key[0, 0].cpu(), exact.to(dtype))
+        assert torch.isfinite(key).all() == (dtype is not torch.float16)
+
+
+def test_lengths_and_starts_outside_their_range():
+    """A length above the table's is cut and reported; one below zero counts as zero and
+    starts outside the query are cut, both without a report."""
+    kp, vp, tables, lens = steered_cache([48, 20], {}, 2, 128, 16, 1.0, 180)
+    q = steered_queries(4, 4, 128, torch.bfloat16, 181)
+    want = q4_cache.attention(q, kp, vp, tables, lens)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = q4_cache.attention(q, kp, vp, tables, ints(48, -2 ** 31))
+    assert torch.equal(got[:2], want[:2]) and not got[2:].any()
+    inside = q4_cache.attention(q, kp, vp, tables, lens, query_starts=ints(0, 2, 4))
+    got = q4_cache.attention(q, kp, vp, tables, lens, query_starts=ints(-5, 2, 2 ** 31 - 1))
+    assert torch.equal(got, inside)
+    assert _lib.device_status(0) == 0
+    tables[1] = tables[0]
+    got = q4_cache.attention(q, kp, vp, tables, ints(48, 2 ** 31 - 1))
+    assert _lib.device_status(0, reset=True) == _lib.KVX_ERR_EXTENT
+    assert torch.equal(got, q4_cache.attention(q, kp, vp, tables, ints(48, 48)))
