@@ -1003,9 +1003,10 @@ __device__ __forceinline__ void store_segment(const AttnArgs& a, const Segment& 
 }
 
 // What bounds it: the bytes of the cache where sequences are long (128 requests of
-// 4096 to 8192 tokens, 8 kv heads: 164 us, 5.25 TB/s, 81% of the card's copy rate;
-// 209 instructions for 16 tokens of a head, half of them unpacking), and what a
-// launch, an item and the join cost where they are short.  Each warp takes its
+// 4096 to 8192 tokens, 8 kv heads: 166 us, 5.2 TB/s, 80% of the card's copy rate)
+// beside the latency of its two warps a scheduler (216 instructions for 16 tokens of a
+// head, 88 of them unpacking, fill half of the issue slots), and what a launch, an
+// item and the join cost where they are short.  Each warp takes its
 // share's segments one after the other, their units in steps through its own ring of two cp.async stages; during a segment's last
 // step the next one's first is on its way already.  Segments that end or begin
 // inside an item leave a partial result in the workspace (at most two for a

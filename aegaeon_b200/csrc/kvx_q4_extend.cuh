@@ -16,7 +16,7 @@
 // the codes, one issues the products.  While one tile's softmax runs, the tensor
 // cores work on the other, and both share the unpacked codes.  (128-row CTAs whose
 // threads did everything in turn, two to an SM, reached 338 TFLOP/s on 1024-token
-// pieces behind 7168 tokens, waiting for loads and for one another; this form 439,
+// pieces behind 7168 tokens, waiting for loads and for one another; this form 443,
 // a quarter of the products' rate.  What bounds it is the softmax: a row's 128
 // scores of a block go through one thread, and the two tiles' products, a fifth of
 // the time, wait for them in turn.)

@@ -201,7 +201,7 @@ std::pair<const char*, const char*> range(const at::Tensor& t) {
 
 // Whether two tensors share bytes (yes, too, where their strides make it too long to tell).
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  const auto ra = range(a), rb = range(b);  // of most pairs they tell: 20 ns
+  const auto ra = range(a), rb = range(b);  // of most pairs they tell
   if (ra.first == ra.second || rb.first == rb.second || ra.second <= rb.first ||
       rb.second <= ra.first)
     return false;
