@@ -523,3 +523,49 @@ def test_lengths_and_starts_outside_their_range():
     got = q4_cache.attention(q, kp, vp, tables, ints(48, 2 ** 31 - 1))
     assert _lib.device_status(0, reset=True) == _lib.KVX_ERR_EXTENT
     assert torch.equal(got, q4_cache.attention(q, kp, vp, tables, ints(48, 48)))
+
+
+# ---- rows keep to themselves ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_query_that_is_no_number_spoils_its_row_alone(bad):
+    for tokens, heads, kv_heads, lens in ((8, 7, 1, [150, 700]), (340, 32, 16, [340])):
+        cache = steered_cache(lens, {}, kv_heads, 128, 16, 1.0, 190)
+        q = steered_queries(tokens, heads, 128, torch.bfloat16, 191)
+        want, want_lse = q4_cache.attention(q, *cache, return_lse=True)
+        q[1, 2, 77] = bad
+        got, lse = q4_cache.attention(q, *cache, return_lse=True)
+        assert got[1, 2].isnan().all() and lse[1, 2].isnan()
+        got[1, 2], lse[1, 2] = want[1, 2], want_lse[1, 2]
+        # Another row's reference point may move earlier or later: a rounding, not the row's number.
+        assert torch.allclose(got.float(), want.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+        assert torch.allclose(lse, want_lse, rtol=0, atol=2.0 ** -18)
+
+
+def test_rows_of_any_size_in_one_tile():
+    """Rows whose scores are far beyond fp32's fractions beside ordinary ones, in one call,
+    and a scale of either sign."""
+    for tokens, heads, kv_heads, lens in ((8, 7, 1, [150, 700]), (340, 32, 16, [340])):
+        cache = steered_cache(lens, {}, kv_heads, 128, 16, 1.0, 195)
+        q = steered_queries(tokens, heads, 128, torch.bfloat16, 196)
+        for scale in (None, -0.05):
+            want, want_lse = q4_cache.attention(q, *cache, scale=scale, return_lse=True)
+            mixed = q.clone()
+            mixed[0::2, 0::3] *= 1e9
+            got, lse = q4_cache.attention(mixed, *cache, scale=scale, return_lse=True)
+            same = torch.ones(q.shape[:2], dtype=torch.bool, device="cuda")
+            same[0::2, 0::3] = False
+            assert torch.isfinite(got).all() and torch.isfinite(lse).all()
+            assert torch.allclose(got[same].float(), want[same].float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+            assert torch.allclose(lse[same], want_lse[same], rtol=0, atol=2.0 ** -18)
+
+
+def test_a_scale_of_zero_is_the_mean():
+    for tokens, heads, kv_heads, lens in ((2, 7, 1, [150, 700]), (340, 32, 16, [340])):
+        cache = steered_cache(lens, {}, kv_heads, 128, 16, 1.0, 197)
+        q = steered_queries(tokens, heads, 128, torch.bfloat16, 198)
+        got, lse = q4_cache.attention(q, *cache, scale=0.0, return_lse=True)
+        want, want_lse, bound, lse_bound = q4_oracle.attention(q, *cache, scale=0.0)
+        assert ((got.double().cpu() - want).abs() <= bound).all()
+        assert ((lse.double().cpu() - want_lse).abs() <= lse_bound).all()
